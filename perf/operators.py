@@ -312,12 +312,10 @@ def own_preference(s):
     if "cfg" not in s:
         kind = {"sigmoid": L.PREF_SIGMOID, "hinge": L.PREF_HINGE, "squared": L.PREF_SQUARED}[c["kind"]]
         s["cfg"] = L.Preference(kind, c["beta"], c["smoothing"], c["margin"], c["mean_tokens"])
-        s["bytes"] = L.preference_loss_workspace(P, S)
-    o = _buffers(s, loss=(P, torch.float32), reward=(2 * P, torch.float32), dlogp=((2 * P, ld), torch.float32),
-                 ws=(s["bytes"], torch.uint8))
+    o = _buffers(s, loss=(P, torch.float32), reward=(2 * P, torch.float32), dlogp=((2 * P, ld), torch.float32))
     L.preference_loss(s["cfg"], s["logp"].data_ptr(), 0 if s["ref"] is None else s["ref"].data_ptr(),
                       s["mask"].data_ptr(), 0, o["loss"].data_ptr(), o["reward"].data_ptr(), o["dlogp"].data_ptr(),
-                      P, S, ld, o["ws"].data_ptr(), s["bytes"], torch.cuda.current_stream().cuda_stream)
+                      P, S, ld, torch.cuda.current_stream().cuda_stream)
     return {"loss": o["loss"], "reward": o["reward"], "dlogp": o["dlogp"][:, :S]}
 
 
@@ -342,10 +340,8 @@ def own_muon(s):
     if "cfg" not in s:
         s["cfg"] = L.Muon(lr=LR, momentum=MU, weight_decay=WD, eps=EPS, nesterov=c["nesterov"],
                           match_rms=c["match_rms"])
-        s["bytes"] = L.muon_update_workspace(c["count"], c["rows"], c["cols"])
-    o = _buffers(s, ws=(s["bytes"], torch.uint8))
     L.muon_update(s["cfg"], s["w"].data_ptr(), s["grad"].data_ptr(), s["momentum"].data_ptr(), c["count"], c["rows"],
-                  c["cols"], o["ws"].data_ptr(), s["bytes"], torch.cuda.current_stream().cuda_stream)
+                  c["cols"], torch.cuda.current_stream().cuda_stream)
     return {"w": s["w"], "momentum": s["momentum"]}
 
 
