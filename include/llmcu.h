@@ -403,6 +403,113 @@ llmcu_status llmcu_attention_bwd_noalloc(const void* q, const void* k, const voi
                                          int batch, int seq, int n_heads, int n_kv_heads, int head_dim,
                                          int ldq, int ldk, int ldv, int lddv, void* stream);
 
+/* ------------------------------------------------- preference tuning
+ * Operators on DEVICE pointers of the current device, next to the kernel-level
+ * entry points above and with their conventions: `stream` is a cudaStream_t,
+ * results are asynchronous, nothing is allocated or kept between calls, a
+ * bounded wait that gave up is reported by llmcu_kernel_checks.  They may be
+ * captured into a CUDA graph.  Calls that may run at the same time need
+ * workspaces of their own; a workspace needs no initial contents and must be
+ * 256-byte aligned (LLMCU_ERR_UNSUPPORTED otherwise).  Sums run in a fixed
+ * order: the same call gives the same bits.  No reference counterpart: the
+ * reference trains with the cross-entropy and AdamW only. */
+
+/* Token log-probabilities of hidden states under a tied head, without logits
+ * in memory: logp[m] = x[m] . E[t] - lse[m] with t = targets[m] and lse[m] =
+ * log sum_v exp(x[m] . E[v]).  x [rows, hidden] and E [vocab, hidden] fp16 with
+ * row strides ldx, lde (elements; multiples of 8 and 16-byte aligned bases, as
+ * the TMA needs, else LLMCU_ERR_UNSUPPORTED); targets int32 [rows]; logp and
+ * lse fp32 [rows].  A target outside [0, vocab) scores nothing: logp is 0 (lse
+ * is the row's all the same).  `workspace` has at least
+ * llmcu_lm_logprobs_workspace(rows, hidden, vocab, 0) bytes. */
+size_t llmcu_lm_logprobs_workspace(int rows, int hidden, int vocab, int backward);
+llmcu_status llmcu_lm_logprobs(const void* x, const void* E, const int32_t* targets, float* logp, float* lse,
+                               int rows, int hidden, int vocab, int ldx, int lde, void* workspace,
+                               size_t workspace_bytes, void* stream);
+/* Its gradient for the hidden states (the head is frozen): dx[m] = scale *
+ * dlogp[m] * (E[t] - sum_v exp(x[m] . E[v] - lse[m]) E[v]) as fp16 [rows,
+ * hidden] with row stride lddx; 0 where the target scores nothing, whatever
+ * dlogp holds there.  lse is the forward's.  `scale` (a loss scale, a power of
+ * two as a rule) keeps small gradients in fp16's range.  Workspace:
+ * llmcu_lm_logprobs_workspace(rows, hidden, vocab, 1) bytes. */
+llmcu_status llmcu_lm_logprobs_bwd(const void* x, const void* E, const int32_t* targets, const float* lse,
+                                   const float* dlogp, void* dx, int rows, int hidden, int vocab, int ldx, int lde,
+                                   int lddx, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Paired preference loss.  Rows i (chosen) and pairs + i (rejected) of the
+ * [2 * pairs, seq] buffers form pair i; R_b is the sum over row b's scored
+ * tokens of logp - ref, or with mean_tokens their mean, D = R_chosen -
+ * R_rejected and h = beta * D - margin:
+ *   LLMCU_PREF_SIGMOID  -(1 - label_smoothing) log s(h) - label_smoothing log s(-h), s the logistic function
+ *   LLMCU_PREF_HINGE    max(0, 1 - h)
+ *   LLMCU_PREF_SQUARED  (D - 1 / (2 beta))^2 */
+typedef enum { LLMCU_PREF_SIGMOID = 0, LLMCU_PREF_HINGE = 1, LLMCU_PREF_SQUARED = 2 } llmcu_pref_kind;
+typedef struct {
+    int32_t kind;          /* llmcu_pref_kind                                       */
+    float beta;            /* > 0                                                   */
+    float label_smoothing; /* in [0, 0.5]; 0 unless LLMCU_PREF_SIGMOID              */
+    float margin;          /* 0 for LLMCU_PREF_SQUARED                              */
+    int32_t mean_tokens;   /* 0 = sums over a row's scored tokens, 1 = their means  */
+} llmcu_preference_cfg;
+/* All buffers [2 * pairs, seq] share the row stride ld (elements, >= seq).
+ * logp fp32; ref_logp fp32 or null (no reference model: 0); mask one byte a
+ * token, non-zero = scored, or null (all are).  What is not scored is not read
+ * (it may hold anything), except that a row without scored tokens has R = 0.
+ * loss [pairs], reward [2 * pairs] (beta * R) and dlogp [2 * pairs, seq] are
+ * fp32 outputs, each nullable.  dlogp is the gradient of sum_i dloss[i] *
+ * loss[i]; dloss fp32 [pairs], null = 1 / pairs (the mean loss).  It is 0 where
+ * nothing is scored; columns from seq to ld are left as they are.  Outputs must
+ * not overlap inputs. */
+llmcu_status llmcu_preference_loss(const llmcu_preference_cfg* cfg, const float* logp, const float* ref_logp,
+                                   const uint8_t* mask, const float* dloss, float* loss, float* reward, float* dlogp,
+                                   int pairs, int seq, int ld, void* stream);
+
+/* Clipped policy loss with a KL term.  Per scored token, with r = exp(logp -
+ * old_logp), advantage A and d = ref_logp - logp:
+ *   obj = min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A), and with dual_clip c where A < 0: max(obj, c A)
+ *   l   = -obj + kl_beta (e^d - d - 1)
+ * and the loss is the mean of l over all scored tokens, the mean over rows of
+ * each row's mean (a row without scored tokens counts 0), or the sum over norm. */
+typedef enum {
+    LLMCU_POLICY_TOKEN_MEAN = 0,
+    LLMCU_POLICY_SEQUENCE_MEAN = 1,
+    LLMCU_POLICY_CONSTANT = 2
+} llmcu_policy_agg;
+typedef struct {
+    float clip_low, clip_high; /* >= 0                                                       */
+    float kl_beta;             /* >= 0; used with a reference only                           */
+    float dual_clip;           /* 0 = off, else > 1                                          */
+    int32_t agg;               /* llmcu_policy_agg                                           */
+    float norm;                /* > 0, LLMCU_POLICY_CONSTANT only                            */
+    int32_t token_advantages;  /* 0 = one advantage per row [batch], 1 = per token, as logp  */
+} llmcu_policy_cfg;
+size_t llmcu_policy_loss_workspace(int batch, int seq);
+/* Buffers [batch, seq] fp32 with row stride ld (>= seq); ref_logp may be null
+ * (no KL term), mask as above.  stats (4 floats) receives the loss, the mean
+ * of e^d - d - 1 over the scored tokens, the share of them that clip, and their
+ * number (exact to 2^24); dlogp (nullable) the loss's gradient, 0 where nothing
+ * is scored.  batch * max(2, (seq + 6) / 4) must stay below 2^31
+ * (LLMCU_ERR_UNSUPPORTED). */
+llmcu_status llmcu_policy_loss(const llmcu_policy_cfg* cfg, const float* logp, const float* old_logp,
+                               const float* ref_logp, const float* advantages, const uint8_t* mask, float* stats,
+                               float* dlogp, int batch, int seq, int ld, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Muon update of `count` matrices [rows, cols] fp32 that follow one another in
+ * w, grad and momentum: momentum = cfg.momentum * momentum + grad; the update u
+ * = grad + cfg.momentum * momentum (nesterov) or momentum; X = u / (|u|_F +
+ * eps), then ns_steps times X = a X + (b X X^T + c (X X^T)^2) X with (a, b, c) =
+ * (3.4445, -4.7750, 2.0315); w = w (1 - lr * weight_decay) - lr * s * X with s =
+ * sqrt(max(1, rows / cols)), or with match_rms 0.2 sqrt(max(rows, cols)).  The
+ * smaller side is at most 16 (the adapters' rank), else LLMCU_ERR_UNSUPPORTED. */
+typedef struct {
+    float lr, momentum, weight_decay, eps;
+    int32_t nesterov, match_rms;
+    int32_t ns_steps; /* 1..16 */
+} llmcu_muon_cfg;
+llmcu_status llmcu_muon_update(const llmcu_muon_cfg* cfg, float* w, const float* grad, float* momentum, int count,
+                               int rows, int cols, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

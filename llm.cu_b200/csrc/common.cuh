@@ -116,7 +116,10 @@ enum class Epi : int {
   kStoreF16Delta = 6,  // fp16 dO + the attention backward's per-(row, head) dO.O sums
   kQKNormRope = 7,     // fp16 q/k/v + (head_dim 128) per-head RMSNorm and RoPE of q and k into rope_out
   kCEStream = 8,       // lm_head forward over one vocabulary chunk: exp(l - ref) into the chunk buffer + partials
+  kLogProb = 9,        // token log-probabilities: per (row, 128-column slot) max and sum, target logits
+  kProbs = 10,         // their backward: 2^kProbShift exp(l - lse) of one vocabulary chunk as fp16
 };
+constexpr float kProbShift = 15.0f;  // kProbs' power of two
 
 struct EpiArgs {
   // generic outputs
@@ -124,6 +127,10 @@ struct EpiArgs {
   int ld_out = 0;
   int accumulate = 0;
   int ksplit = 1;  // kStoreF32 with accumulate: K slices that reduce-add into the same output
+  // kStoreF32 with ksplit > 1: rows between the K slices' own outputs (a
+  // multiple of 256; out then has ksplit * slab_rows rows and each element one
+  // writer, so the sums' order is fixed; no accumulate needed); 0: the same rows
+  int slab_rows = 0;
   // kStoreF16Delta: O [M, n_main] (row stride ld_o) and the delta output [B, n_heads, seq]
   const __half* attn_o = nullptr;
   int ld_o = 0;
@@ -162,6 +169,9 @@ struct EpiArgs {
   const float* ce_ref = nullptr;
   int vocab_off = 0;
   int ce_slots = 0;
+  // kLogProb: (max, sum) per (slot, row), [slots, M]; kProbs: lse [M]
+  float2* part2 = nullptr;
+  const float* lse = nullptr;
 };
 
 // C[M,N] = A . B^T (B K-major) or A . B (B MN-major) with the given
@@ -255,5 +265,75 @@ cudaError_t quantize_rows_int8(const float* w, int rows, int cols, int8_t* q, fl
 // kernels' bounded-wait limit and ORs kErrWaitProducer into err.
 cudaError_t wait_selftest(int* err, cudaStream_t st);
 cudaError_t dequant_rows_f16(const int8_t* q, const float* scale, int rows, int cols, __half* out, cudaStream_t st);
+
+// ---- logprobs.cu (x [M, H], E [V, H] fp16 with row strides ldx, lde; targets
+// outside [0, V) score nothing: logp 0, dx row 0)
+size_t lm_logprobs_workspace(int M, int H, int V, bool backward);
+cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, float* logp, float* lse, int M, int H,
+                        int V, int ldx, int lde, void* ws, int* err, cudaStream_t st);
+cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* targets, const float* lse,
+                                 const float* dlogp, __half* dx, int M, int H, int V, int ldx, int lde, int lddx,
+                                 float scale, void* ws, int* err, cudaStream_t st);
+
+// ---- losses.cu: all pointers but the ones marked nullable are required
+enum PrefKind : int { kPrefSigmoid = 0, kPrefHinge = 1, kPrefSquared = 2 };
+struct PreferenceArgs {
+  const float *logp, *ref;  // [2 * pairs, ld]; ref nullable (0)
+  const uint8_t* mask;      // [2 * pairs, ld]; nullable (all scored)
+  const float* dloss;       // [pairs] upstream gradients; nullable (1 / pairs)
+  float *loss, *reward;     // [pairs], [2 * pairs]; nullable
+  float* dlogp;             // [2 * pairs, ld]; nullable
+  int pairs, seq, ld;
+  int kind, mean_tokens;
+  float beta, smoothing, margin;
+  bool vec;     // set by preference_loss: aligned bases
+  int cluster;  // set by preference_loss
+};
+cudaError_t preference_loss(PreferenceArgs a, cudaStream_t st);
+
+enum PolicyAgg : int { kPolicyTokenMean = 0, kPolicySequenceMean = 1, kPolicyConstant = 2 };
+struct PolicyArgs {
+  const float *logp, *old, *ref;  // [batch, ld]; ref nullable (no KL term)
+  const float* adv;               // [batch], or [batch, ld] with token_adv
+  const uint8_t* mask;            // [batch, ld]; nullable
+  float* stats;                   // [4]
+  float* dlogp;                   // [batch, ld]; nullable
+  int batch, seq, ld;
+  int agg, token_adv;
+  float beta, inv_norm;                // inv_norm: kPolicyConstant
+  float low, high, dual;               // the clip's bounds on r (dual: on r for A < 0)
+  double log_low, log_high, log_dual;  // their logarithms; -inf / inf where there is none
+  // set by policy_loss
+  bool vec;
+  int row_quads;
+  int64_t units;
+  uint32_t div_m;
+  int div_s;
+};
+size_t policy_loss_workspace(int batch);
+cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st);
+
+// ---- muon.cu
+constexpr int kMuonMaxRank = 16;  // the smaller side of every matrix
+constexpr int kMuonMaxSlots = 14;
+struct MuonSlot {
+  int64_t off;  // in floats, from the start of a layer
+  int rows, cols;
+};
+// `layers` sets of the slots' matrices, layer_stride floats apart, at the same
+// places of w, grad and mom.
+struct MuonArgs {
+  float* w;
+  const float* grad;
+  float* mom;
+  MuonSlot slot[kMuonMaxSlots];
+  int n_slots, layers;
+  int64_t layer_stride;
+  float lr, momentum, weight_decay, eps;
+  int nesterov, match_rms, steps;
+  // set by muon_update
+  int cluster, tile, pitch;
+};
+cudaError_t muon_update(MuonArgs a, cudaStream_t st);
 
 }  // namespace llmcu

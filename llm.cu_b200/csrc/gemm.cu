@@ -202,6 +202,20 @@ cudaError_t dispatch(Epi epi, const EpiArgs& ea, const CUtensorMap* maps, const 
       } else {
         return cudaErrorInvalidValue;
       }
+    case Epi::kLogProb:
+      if constexpr (BN == 256 && !BMN) {
+        return launch<BN, EpiLogProb, BMN, CG>(maps, sh, EpiLogProb::Params{ea.targets, ea.part2, ea.tgt_logit}, err,
+                                               st);
+      } else {
+        return cudaErrorInvalidValue;
+      }
+    case Epi::kProbs:
+      if constexpr (BN == 256 && !BMN) {
+        return launch<BN, EpiProbs, BMN, CG>(maps, sh, EpiProbs::Params{ea.targets, ea.lse, ea.tgt_logit, ea.vocab_off},
+                                             err, st);
+      } else {
+        return cudaErrorInvalidValue;
+      }
   }
   return cudaErrorInvalidValue;
 }
@@ -275,7 +289,10 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
   if (epi == Epi::kCEStream && (!ea.targets || !ea.ce_ref || !ea.part_max || !ea.part_sum || !ea.tgt_logit ||
                                 ea.vocab_off % 128 || ea.ce_slots < (ea.vocab_off + N + 127) / 128))
     return cudaErrorInvalidValue;
-  if (ea.ksplit > 1 && (epi != Epi::kStoreF32 || !ea.accumulate)) return cudaErrorInvalidValue;
+  if (epi == Epi::kLogProb && (BN != 256 || !ea.targets || !ea.part2 || !ea.tgt_logit)) return cudaErrorInvalidValue;
+  if (epi == Epi::kProbs && (BN != 256 || !ea.targets || !ea.lse || !ea.tgt_logit)) return cudaErrorInvalidValue;
+  if (ea.ksplit > 1 && (epi != Epi::kStoreF32 || (!ea.accumulate && !ea.slab_rows))) return cudaErrorInvalidValue;
+  if (ea.slab_rows && (ea.slab_rows % (2 * kBlockM) || ea.slab_rows < M)) return cudaErrorInvalidValue;
   const int n_main = ea.n_main > 0 ? ea.n_main : N;
   if (n_main < N) {  // side output: only for the plain stores, from a tile boundary
     if ((epi != Epi::kStoreF16 && epi != Epi::kStoreF16Delta && epi != Epi::kResidF32 &&
@@ -298,6 +315,7 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
     case Epi::kStoreF16:
     case Epi::kStoreF16Delta:
     case Epi::kCEStream:
+    case Epi::kProbs:
       okc = make_io_map(&maps[2], ea.out, M, n_main, ea.ld_out, false);
       maps[3] = maps[2];
       break;
@@ -305,8 +323,11 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
       okc = make_io_map(&maps[2], ea.out, M, n_main, ea.ld_out, false) &&
             make_io_map(&maps[3], ea.rope_out, M, ea.n_qk_cols, ea.ld_rope, false);
       break;
+    case Epi::kLogProb:  // nothing leaves through a map
+      maps[2] = maps[3] = maps[0];
+      break;
     case Epi::kStoreF32:
-      okc = make_io_map(&maps[2], ea.out, M, N, ea.ld_out, true);
+      okc = make_io_map(&maps[2], ea.out, ea.slab_rows ? ea.ksplit * ea.slab_rows : M, N, ea.ld_out, true);
       maps[3] = maps[2];
       break;
     case Epi::kResidF32:
@@ -347,7 +368,8 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
     const int kbps = (nk + ea.ksplit - 1) / ea.ksplit;
     sh.kb_per_split = kbps;
     sh.splits = (nk + kbps - 1) / kbps;
-  } else if (t_fx_ws && epi != Epi::kCEStream) {
+    sh.split_row_tiles = ea.slab_rows / (kBlockM * CG);
+  } else if (t_fx_ws && epi != Epi::kCEStream && epi != Epi::kLogProb && epi != Epi::kProbs) {
     // tiles that fill under half a wave: K splits with a fix-up, about one
     // wave of units, at least two 64-deep K blocks each
     const int slots = CG == 2 ? g_num_sms / 2 : g_num_sms;

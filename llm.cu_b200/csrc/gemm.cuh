@@ -843,6 +843,130 @@ struct EpiCEStream {
   __device__ static void end(State&, const Params&, const EpiCtx&, int) {}
 };
 
+// Token log-probabilities, forward (lm_logprobs): per row and 128-column slot
+// of the vocabulary the pair (m, sum of exp(l - m)), m the slot's maximum, and
+// the target's logit; the logits themselves go nowhere.  The pairs lie
+// [slot][row], so a warp's 32 rows store 256 contiguous bytes.  A row whose
+// slot is all -inf leaves (-inf, 0).
+struct EpiLogProb {
+  struct Params {
+    const int* targets;  // [M]
+    float2* part;        // [slots, M]
+    float* tgt_logit;    // [M]
+  };
+  struct State {};
+  static constexpr int kChunk = 128;
+  static constexpr int kSlab = 0;
+  static constexpr bool kPaired = false;
+  static constexpr bool kStores = false;
+  static constexpr bool kTmemDirect = true;
+  __device__ static void begin(State&, const Params&, const EpiCtx&, int) {}
+  __device__ static bool tile(State&, const Params& p, EpiCtx& c, int col0, uint32_t taddr, int) {
+    if (col0 >= c.N) return true;
+    const int nv = min(128, c.N - col0);
+    const bool live = c.row < c.M;
+    const int t = live ? __ldg(p.targets + c.row) - col0 : -1;
+    // a whole slot without any of the warp's targets (nearly every slot): no per-column tests
+    const bool plain = nv == 128 && !__any_sync(0xffffffffu, t >= 0 && t < 128);
+    float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {  // 32 columns at a time: running maximum and sum
+      float v[32];
+      tmem_ld_32x32b_x32(taddr + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(v));
+      tmem_ld_wait();
+      if (!plain) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          if (32 * q + j == t) p.tgt_logit[c.row] = v[j];
+          if (32 * q + j >= nv) v[j] = -INFINITY;
+        }
+      }
+      float mq = m;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) mq = fmaxf(mq, v[j]);
+      if (mq > -INFINITY) {
+        const float r2 = mq * kLog2e;
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          a += fast_exp2(fmaf(v[j], kLog2e, -r2));
+          b += fast_exp2(fmaf(v[j + 1], kLog2e, -r2));
+        }
+        s = fmaf(s, fast_exp2(fmaf(m, kLog2e, -r2)), a + b);
+        m = mq;
+      } else {  // -inf so far, or NaN among -inf: the sum keeps the NaN
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s += v[j] == -INFINITY ? 0.f : v[j];
+      }
+    }
+    if (live) p.part[static_cast<size_t>(col0 >> 7) * c.M + c.row] = make_float2(m, s);
+    return true;
+  }
+  __device__ static void end(State&, const Params&, const EpiCtx&, int) {}
+};
+
+// Token log-probabilities, backward (lm_logprobs_backward), one vocabulary
+// chunk: 2^15 exp(l - lse) as fp16 into the chunk buffer (mapC).  lse is
+// known, so no value passes 2^15 and the factor keeps probabilities down to
+// 2^-29 (a uniform distribution over 150 k ids is at 2^-17) in fp16's normal
+// range.  The rounding to fp16 (at most 2^-11 of each value) is what the
+// tensor cores' product with E needs; the target's column, whose p - 1 it
+// would spoil for a confident token, is stored as 0 and added in fp32 by the
+// finishing kernel, which takes its logit from here.
+struct EpiProbs {
+  struct Params {
+    const int* targets;  // [M]
+    const float* lse;    // [M]
+    float* tgt_logit;    // [M]
+    int vocab_off;       // vocabulary index of the chunk's column 0
+  };
+  struct State {};
+  static constexpr int kChunk = 128;
+  static constexpr int kSlab = kSlabBytes;
+  static constexpr bool kPaired = false;
+  static constexpr bool kStores = true;
+  static constexpr bool kTmemDirect = true;
+  __device__ static void begin(State&, const Params&, const EpiCtx&, int) {}
+  __device__ static bool tile(State&, const Params& p, EpiCtx& c, int col0, uint32_t taddr, int) {
+    if (col0 >= c.N) return true;
+    const int nv = min(128, c.N - col0);
+    const bool live = c.row < c.M;
+    const int t = live ? __ldg(p.targets + c.row) - (p.vocab_off + col0) : -1;
+    const float off = live ? kProbShift - __ldg(p.lse + c.row) * kLog2e : 0.f;
+    const bool plain = nv == 128 && !__any_sync(0xffffffffu, t >= 0 && t < 128);
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {  // 64 columns = one 128-byte slab row of fp16
+      if (64 * h >= nv) break;
+      uint32_t pk[32];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float v[32];
+        tmem_ld_32x32b_x32(taddr + 64 * h + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(v));
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          float e0 = fast_exp2(fmaf(v[j], kLog2e, off));
+          float e1 = fast_exp2(fmaf(v[j + 1], kLog2e, off));
+          if (!plain) {
+            const int cj = 64 * h + 32 * q + j;
+            if (cj == t) p.tgt_logit[c.row] = v[j];
+            if (cj + 1 == t) p.tgt_logit[c.row] = v[j + 1];
+            if (cj >= nv || cj == t) e0 = 0.f;
+            if (cj + 1 >= nv || cj + 1 == t) e1 = 0.f;
+          }
+          pk[16 * q + j / 2] = pack_half2(e0, e1);
+        }
+      }
+      slab_wait_read(c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) slab_st(c, j, make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]));
+      slab_store(c, c.mapC, col0 + 64 * h, c.row0);
+    }
+    return true;
+  }
+  __device__ static void end(State&, const Params&, const EpiCtx&, int) {}
+};
+
 // begin(st, p, c, slot, col0): the epilogue takes its slice's first column
 template <class E, class = void>
 struct epi_begin_col : std::false_type {};

@@ -28,6 +28,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 #include <thread>
 #include <vector>
@@ -2001,6 +2002,165 @@ llmcu_status llmcu_attention_bwd(const void* q, const void* k, const void* v, co
       static_cast<__half*>(dv), batch, seq, n_heads, n_kv_heads, head_dim, ldq, ldk, ldv, ldo, ldo,
       n_kv_heads * head_dim, lddv, d_err, static_cast<cudaStream_t>(stream));
   return kernel_status(e);
+}
+
+// ------------------------------------------------------ preference tuning
+
+size_t llmcu_lm_logprobs_workspace(int rows, int hidden, int vocab, int backward) {
+  if (rows <= 0 || hidden <= 0 || vocab <= 0) return 0;
+  return lm_logprobs_workspace(rows, hidden, vocab, backward != 0);
+}
+
+static bool bad_workspace(const void* ws) { return reinterpret_cast<uintptr_t>(ws) % 256 != 0; }
+static bool bad_floats(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % 4) return true;
+  return false;
+}
+
+llmcu_status llmcu_lm_logprobs(const void* x, const void* E, const int32_t* targets, float* logp, float* lse, int rows,
+                               int hidden, int vocab, int ldx, int lde, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  if (!x || !E || !targets || !logp || !lse || !workspace || rows <= 0 || hidden <= 0 || vocab <= 0 || ldx < hidden ||
+      lde < hidden || workspace_bytes < lm_logprobs_workspace(rows, hidden, vocab, false))
+    return LLMCU_ERR_INVALID_ARG;
+  if (bad_workspace(workspace) || bad_floats({targets, logp, lse})) return LLMCU_ERR_UNSUPPORTED;
+  int* d_err = nullptr;
+  if (kernel_err_word(&d_err) != cudaSuccess) return LLMCU_ERR_CUDA;
+  return kernel_status(lm_logprobs(static_cast<const __half*>(x), static_cast<const __half*>(E), targets, logp, lse,
+                                   rows, hidden, vocab, ldx, lde, workspace, d_err,
+                                   static_cast<cudaStream_t>(stream)));
+}
+
+llmcu_status llmcu_lm_logprobs_bwd(const void* x, const void* E, const int32_t* targets, const float* lse,
+                                   const float* dlogp, void* dx, int rows, int hidden, int vocab, int ldx, int lde,
+                                   int lddx, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!x || !E || !targets || !lse || !dlogp || !dx || !workspace || rows <= 0 || hidden <= 0 || vocab <= 0 ||
+      ldx < hidden || lde < hidden || lddx < hidden ||
+      workspace_bytes < lm_logprobs_workspace(rows, hidden, vocab, true))
+    return LLMCU_ERR_INVALID_ARG;
+  if (bad_workspace(workspace) || bad_floats({targets, lse, dlogp}) || reinterpret_cast<uintptr_t>(dx) % 2)
+    return LLMCU_ERR_UNSUPPORTED;
+  int* d_err = nullptr;
+  if (kernel_err_word(&d_err) != cudaSuccess) return LLMCU_ERR_CUDA;
+  return kernel_status(lm_logprobs_backward(static_cast<const __half*>(x), static_cast<const __half*>(E), targets, lse,
+                                            dlogp, static_cast<__half*>(dx), rows, hidden, vocab, ldx, lde, lddx, scale,
+                                            workspace, d_err, static_cast<cudaStream_t>(stream)));
+}
+
+static bool preference_args(const llmcu_preference_cfg* cfg, PreferenceArgs* a) {
+  if (!cfg || cfg->kind < LLMCU_PREF_SIGMOID || cfg->kind > LLMCU_PREF_SQUARED || !(cfg->beta > 0.f) ||
+      !std::isfinite(cfg->beta) || !(cfg->label_smoothing >= 0.f && cfg->label_smoothing <= 0.5f) ||
+      (cfg->label_smoothing != 0.f && cfg->kind != LLMCU_PREF_SIGMOID) || !std::isfinite(cfg->margin) ||
+      (cfg->margin != 0.f && cfg->kind == LLMCU_PREF_SQUARED) || (cfg->mean_tokens != 0 && cfg->mean_tokens != 1))
+    return false;
+  a->kind = cfg->kind;
+  a->beta = cfg->beta;
+  a->smoothing = cfg->label_smoothing;
+  a->margin = cfg->margin;
+  a->mean_tokens = cfg->mean_tokens;
+  return true;
+}
+
+llmcu_status llmcu_preference_loss(const llmcu_preference_cfg* cfg, const float* logp, const float* ref_logp,
+                                   const uint8_t* mask, const float* dloss, float* loss, float* reward, float* dlogp,
+                                   int pairs, int seq, int ld, void* stream) {
+  PreferenceArgs a{};
+  if (!preference_args(cfg, &a) || !logp || pairs <= 0 || pairs > (1 << 27) || seq <= 0 || ld < seq)
+    return LLMCU_ERR_INVALID_ARG;
+  if (bad_floats({logp, ref_logp, dloss, loss, reward, dlogp})) return LLMCU_ERR_UNSUPPORTED;
+  a.logp = logp;
+  a.ref = ref_logp;
+  a.mask = mask;
+  a.dloss = dloss;
+  a.loss = loss;
+  a.reward = reward;
+  a.dlogp = dlogp;
+  a.pairs = pairs;
+  a.seq = seq;
+  a.ld = ld;
+  return kernel_status(preference_loss(a, static_cast<cudaStream_t>(stream)));
+}
+
+static bool policy_args(const llmcu_policy_cfg* cfg, PolicyArgs* a) {
+  if (!cfg || !(cfg->clip_low >= 0.f) || !(cfg->clip_high >= 0.f) || !std::isfinite(cfg->clip_low) ||
+      !std::isfinite(cfg->clip_high) || !(cfg->kl_beta >= 0.f) || !std::isfinite(cfg->kl_beta) ||
+      !(cfg->dual_clip == 0.f || cfg->dual_clip > 1.f) || !std::isfinite(cfg->dual_clip) ||
+      cfg->agg < LLMCU_POLICY_TOKEN_MEAN || cfg->agg > LLMCU_POLICY_CONSTANT ||
+      (cfg->agg == LLMCU_POLICY_CONSTANT && (!(cfg->norm > 0.f) || !std::isfinite(cfg->norm))) ||
+      (cfg->token_advantages != 0 && cfg->token_advantages != 1))
+    return false;
+  a->agg = cfg->agg;
+  a->token_adv = cfg->token_advantages;
+  a->beta = cfg->kl_beta;
+  a->inv_norm = cfg->agg == LLMCU_POLICY_CONSTANT ? static_cast<float>(1.0 / cfg->norm) : 0.f;
+  const double low = 1.0 - cfg->clip_low, high = 1.0 + cfg->clip_high;
+  a->low = static_cast<float>(low);
+  a->high = static_cast<float>(high);
+  a->dual = cfg->dual_clip;
+  // a ratio is never below 1 - clip_low where that is 0 or less
+  a->log_low = low > 0.0 ? std::log1p(-static_cast<double>(cfg->clip_low)) : -INFINITY;
+  a->log_high = std::log1p(static_cast<double>(cfg->clip_high));
+  a->log_dual = cfg->dual_clip > 0.f ? std::log(static_cast<double>(cfg->dual_clip)) : INFINITY;
+  return true;
+}
+
+size_t llmcu_policy_loss_workspace(int batch, int seq) {
+  return batch > 0 && seq > 0 ? policy_loss_workspace(batch) : 0;
+}
+
+llmcu_status llmcu_policy_loss(const llmcu_policy_cfg* cfg, const float* logp, const float* old_logp,
+                               const float* ref_logp, const float* advantages, const uint8_t* mask, float* stats,
+                               float* dlogp, int batch, int seq, int ld, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  PolicyArgs a{};
+  if (!policy_args(cfg, &a) || !logp || !old_logp || !advantages || !stats || !workspace || batch <= 0 || seq <= 0 ||
+      ld < seq || workspace_bytes < policy_loss_workspace(batch))
+    return LLMCU_ERR_INVALID_ARG;
+  if (bad_workspace(workspace) || bad_floats({logp, old_logp, ref_logp, advantages, stats, dlogp}))
+    return LLMCU_ERR_UNSUPPORTED;
+  a.logp = logp;
+  a.old = old_logp;
+  a.ref = ref_logp;
+  a.adv = advantages;
+  a.mask = mask;
+  a.stats = stats;
+  a.dlogp = dlogp;
+  a.batch = batch;
+  a.seq = seq;
+  a.ld = ld;
+  return kernel_status(policy_loss(a, workspace, static_cast<cudaStream_t>(stream)));
+}
+
+static bool muon_args(const llmcu_muon_cfg* cfg, MuonArgs* a) {
+  if (!cfg || !std::isfinite(cfg->lr) || !std::isfinite(cfg->momentum) || !std::isfinite(cfg->weight_decay) ||
+      !(cfg->eps > 0.f) || !std::isfinite(cfg->eps) || cfg->ns_steps < 1 || cfg->ns_steps > 16 ||
+      (cfg->nesterov != 0 && cfg->nesterov != 1) || (cfg->match_rms != 0 && cfg->match_rms != 1))
+    return false;
+  a->lr = cfg->lr;
+  a->momentum = cfg->momentum;
+  a->weight_decay = cfg->weight_decay;
+  a->eps = cfg->eps;
+  a->nesterov = cfg->nesterov;
+  a->match_rms = cfg->match_rms;
+  a->steps = cfg->ns_steps;
+  return true;
+}
+
+llmcu_status llmcu_muon_update(const llmcu_muon_cfg* cfg, float* w, const float* grad, float* momentum, int count,
+                               int rows, int cols, void* stream) {
+  MuonArgs a{};
+  if (!muon_args(cfg, &a) || !w || !grad || !momentum || count <= 0 || rows <= 0 || cols <= 0)
+    return LLMCU_ERR_INVALID_ARG;
+  if (bad_floats({w, grad, momentum})) return LLMCU_ERR_UNSUPPORTED;
+  a.w = w;
+  a.grad = grad;
+  a.mom = momentum;
+  a.slot[0] = MuonSlot{0, rows, cols};
+  a.n_slots = 1;
+  a.layers = count;
+  a.layer_stride = static_cast<int64_t>(rows) * cols;
+  return kernel_status(muon_update(a, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 from dataclasses import dataclass
+from functools import cached_property
 from typing import Optional
 
 import numpy as np
@@ -42,6 +43,8 @@ def targets_mask(names) -> int:
         m |= 1 << ids[n]
     return m
 BASE_FP16, BASE_INT8 = 0, 1
+PREF_SIGMOID, PREF_HINGE, PREF_SQUARED = range(3)
+POLICY_TOKEN_MEAN, POLICY_SEQUENCE_MEAN, POLICY_CONSTANT = range(3)
 
 
 class LlmcuError(RuntimeError):
@@ -74,6 +77,21 @@ class _LoraLayout(C.Structure):
 class _AdamWCfg(C.Structure):
     _fields_ = [("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float),
                 ("weight_decay", C.c_float)]
+
+
+class _PreferenceCfg(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("beta", C.c_float), ("label_smoothing", C.c_float), ("margin", C.c_float),
+                ("mean_tokens", C.c_int32)]
+
+
+class _PolicyCfg(C.Structure):
+    _fields_ = [("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_beta", C.c_float), ("dual_clip", C.c_float),
+                ("agg", C.c_int32), ("norm", C.c_float), ("token_advantages", C.c_int32)]
+
+
+class _MuonCfg(C.Structure):
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("eps", C.c_float),
+                ("nesterov", C.c_int32), ("match_rms", C.c_int32), ("ns_steps", C.c_int32)]
 
 
 @dataclass(frozen=True)
@@ -127,6 +145,54 @@ class AdamW:
     weight_decay: float = 0.01
 
 
+@dataclass(frozen=True)
+class Preference:
+    """Paired preference loss (llmcu_preference_cfg)."""
+    kind: int = PREF_SIGMOID
+    beta: float = 0.1
+    label_smoothing: float = 0.0
+    margin: float = 0.0
+    mean_tokens: bool = False
+
+    @cached_property
+    def c(self):
+        return _PreferenceCfg(self.kind, self.beta, self.label_smoothing, self.margin, int(self.mean_tokens))
+
+
+@dataclass(frozen=True)
+class Policy:
+    """Clipped policy loss with a KL term (llmcu_policy_cfg)."""
+    clip_low: float = 0.2
+    clip_high: float = 0.2
+    kl_beta: float = 0.0
+    dual_clip: float = 0.0
+    agg: int = POLICY_TOKEN_MEAN
+    norm: float = 1.0             # POLICY_CONSTANT only
+    token_advantages: bool = False
+
+    @cached_property
+    def c(self):
+        return _PolicyCfg(self.clip_low, self.clip_high, self.kl_beta, self.dual_clip, self.agg, self.norm,
+                          int(self.token_advantages))
+
+
+@dataclass(frozen=True)
+class Muon:
+    """Momentum with the update orthogonalised by Newton-Schulz steps (llmcu_muon_cfg)."""
+    lr: float = 2e-2
+    momentum: float = 0.95
+    weight_decay: float = 0.0
+    eps: float = 1e-7
+    nesterov: bool = True
+    match_rms: bool = False
+    ns_steps: int = 5
+
+    @cached_property
+    def c(self):
+        return _MuonCfg(self.lr, self.momentum, self.weight_decay, self.eps, int(self.nesterov), int(self.match_rms),
+                        self.ns_steps)
+
+
 _lib: Optional[C.CDLL] = None
 
 _SIGS = {
@@ -175,6 +241,15 @@ _SIGS = {
     "llmcu_attention_fwd": (C.c_int, [C.c_void_p] * 5 + [C.c_int] * 8 + [C.c_void_p]),
     "llmcu_attention_bwd": (C.c_int, [C.c_void_p] * 10 + [C.c_int] * 9 + [C.c_void_p]),
     "llmcu_attention_bwd_noalloc": (C.c_int, [C.c_void_p] * 9 + [C.c_int] * 9 + [C.c_void_p]),
+    "llmcu_lm_logprobs_workspace": (C.c_size_t, [C.c_int] * 4),
+    "llmcu_lm_logprobs": (C.c_int, [C.c_void_p] * 5 + [C.c_int] * 5 + [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "llmcu_lm_logprobs_bwd": (C.c_int, [C.c_void_p] * 6 + [C.c_int] * 6 + [C.c_float, C.c_void_p, C.c_size_t,
+                                                                           C.c_void_p]),
+    "llmcu_preference_loss": (C.c_int, [C.POINTER(_PreferenceCfg)] + [C.c_void_p] * 7 + [C.c_int] * 3 + [C.c_void_p]),
+    "llmcu_policy_loss_workspace": (C.c_size_t, [C.c_int] * 2),
+    "llmcu_policy_loss": (C.c_int, [C.POINTER(_PolicyCfg)] + [C.c_void_p] * 7 + [C.c_int] * 3 +
+                          [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "llmcu_muon_update": (C.c_int, [C.POINTER(_MuonCfg)] + [C.c_void_p] * 3 + [C.c_int] * 3 + [C.c_void_p]),
     "llmcu_kernel_checks": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
     "llmcu_kernel_wait_selftest": (C.c_int, [C.c_void_p]),
     "llmcu_lora_layout_count": (C.c_int64, [C.POINTER(_LoraLayout)]),
@@ -543,3 +618,40 @@ def kernel_wait_selftest(stream=0):
 
 def quantize_int8_rows(w_ptr, rows, cols, q_ptr, scale_ptr, stream=0):
     _chk(lib().llmcu_quantize_int8_rows(w_ptr, rows, cols, q_ptr, scale_ptr, stream), "quantize_int8_rows")
+
+
+def lm_logprobs_workspace(rows, hidden, vocab, backward=False) -> int:
+    """Bytes of workspace of lm_logprobs (or, backward, of lm_logprobs_bwd)."""
+    return int(lib().llmcu_lm_logprobs_workspace(rows, hidden, vocab, int(backward)))
+
+
+def lm_logprobs(x, E, targets, logp, lse, rows, hidden, vocab, ldx, lde, workspace, workspace_bytes, stream=0):
+    _chk(lib().llmcu_lm_logprobs(x, E, targets, logp, lse, rows, hidden, vocab, ldx, lde, workspace, workspace_bytes,
+                                 stream), "lm_logprobs")
+
+
+def lm_logprobs_bwd(x, E, targets, lse, dlogp, dx, rows, hidden, vocab, ldx, lde, lddx, scale, workspace,
+                    workspace_bytes, stream=0):
+    _chk(lib().llmcu_lm_logprobs_bwd(x, E, targets, lse, dlogp, dx, rows, hidden, vocab, ldx, lde, lddx, scale,
+                                     workspace, workspace_bytes, stream), "lm_logprobs_bwd")
+
+
+def preference_loss(cfg: Preference, logp, ref_logp, mask, dloss, loss, reward, dlogp, pairs, seq, ld, stream=0):
+    """0 for ref_logp, mask, dloss or an output leaves it out (see llmcu.h)."""
+    _chk(lib().llmcu_preference_loss(cfg.c, logp, ref_logp, mask, dloss, loss, reward, dlogp, pairs, seq, ld, stream),
+         "preference_loss")
+
+
+def policy_loss_workspace(batch, seq) -> int:
+    return int(lib().llmcu_policy_loss_workspace(batch, seq))
+
+
+def policy_loss(cfg: Policy, logp, old_logp, ref_logp, advantages, mask, stats, dlogp, batch, seq, ld, workspace,
+                workspace_bytes, stream=0):
+    """0 for ref_logp, mask or dlogp leaves it out; stats: loss, mean KL, share clipped, tokens (see llmcu.h)."""
+    _chk(lib().llmcu_policy_loss(cfg.c, logp, old_logp, ref_logp, advantages, mask, stats, dlogp, batch, seq, ld,
+                                 workspace, workspace_bytes, stream), "policy_loss")
+
+
+def muon_update(cfg: Muon, w, grad, momentum, count, rows, cols, stream=0):
+    _chk(lib().llmcu_muon_update(cfg.c, w, grad, momentum, count, rows, cols, stream), "muon_update")
