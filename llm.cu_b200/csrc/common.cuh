@@ -58,6 +58,24 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// Launch `kern` in clusters of C CTAs (grid: a multiple of C).
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_cluster(void (*kern)(KArgs...), unsigned grid, int block, int C, size_t smem, cudaStream_t st,
+                                  Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = C;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
 
 // ---- attention.cu
 cudaError_t attention_forward(const __half* q, const __half* k, const __half* v, __half* o, float* lse, int B, int S,
@@ -304,6 +322,8 @@ struct PolicyArgs {
   float low, high, dual;               // the clip's bounds on r (dual: on r for A < 0)
   double log_low, log_high, log_dual;  // their logarithms; -inf / inf where there is none
   // set by policy_loss
+  float f_low, f_high, f_dual;  // the logarithms in fp32
+  float near;                   // distance to one of them that fp32 does not resolve
   bool vec;
   int row_quads;
   int64_t units;

@@ -211,7 +211,7 @@ cudaError_t dispatch(Epi epi, const EpiArgs& ea, const CUtensorMap* maps, const 
       }
     case Epi::kProbs:
       if constexpr (BN == 256 && !BMN) {
-        return launch<BN, EpiProbs, BMN, CG>(maps, sh, EpiProbs::Params{ea.targets, ea.lse, ea.tgt_logit, ea.vocab_off},
+        return launch<BN, EpiProbs, BMN, CG>(maps, sh, EpiProbs::Params{ea.targets, ea.lse, ea.vocab_off},
                                              err, st);
       } else {
         return cudaErrorInvalidValue;
@@ -290,7 +290,7 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
                                 ea.vocab_off % 128 || ea.ce_slots < (ea.vocab_off + N + 127) / 128))
     return cudaErrorInvalidValue;
   if (epi == Epi::kLogProb && (BN != 256 || !ea.targets || !ea.part2 || !ea.tgt_logit)) return cudaErrorInvalidValue;
-  if (epi == Epi::kProbs && (BN != 256 || !ea.targets || !ea.lse || !ea.tgt_logit)) return cudaErrorInvalidValue;
+  if (epi == Epi::kProbs && (BN != 256 || !ea.targets || !ea.lse)) return cudaErrorInvalidValue;
   if (ea.ksplit > 1 && (epi != Epi::kStoreF32 || (!ea.accumulate && !ea.slab_rows))) return cudaErrorInvalidValue;
   if (ea.slab_rows && (ea.slab_rows % (2 * kBlockM) || ea.slab_rows < M)) return cudaErrorInvalidValue;
   const int n_main = ea.n_main > 0 ? ea.n_main : N;

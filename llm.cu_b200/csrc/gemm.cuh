@@ -912,12 +912,11 @@ struct EpiLogProb {
 // range.  The rounding to fp16 (at most 2^-11 of each value) is what the
 // tensor cores' product with E needs; the target's column, whose p - 1 it
 // would spoil for a confident token, is stored as 0 and added in fp32 by the
-// finishing kernel, which takes its logit from here.
+// finishing kernel.
 struct EpiProbs {
   struct Params {
     const int* targets;  // [M]
     const float* lse;    // [M]
-    float* tgt_logit;    // [M]
     int vocab_off;       // vocabulary index of the chunk's column 0
   };
   struct State {};
@@ -949,8 +948,6 @@ struct EpiProbs {
           float e1 = fast_exp2(fmaf(v[j + 1], kLog2e, off));
           if (!plain) {
             const int cj = 64 * h + 32 * q + j;
-            if (cj == t) p.tgt_logit[c.row] = v[j];
-            if (cj + 1 == t) p.tgt_logit[c.row] = v[j + 1];
             if (cj >= nv || cj == t) e0 = 0.f;
             if (cj + 1 >= nv || cj + 1 == t) e1 = 0.f;
           }

@@ -18,19 +18,55 @@ namespace llmcu {
 
 namespace {
 
+// x . e in fp32 by one warp (the same order of sums wherever it is called):
+// the target's logit.  The tensor cores cut what they add to the accumulator,
+// which leaves a logit of 10 about 3e-5 short after 128 steps of K; over the
+// sum of the exponentials that hardly shows, in l_t - lse it does.
+__device__ __forceinline__ float target_logit(const __half* __restrict__ x, const __half* __restrict__ e, int H,
+                                              int lane) {
+  float s = 0.f;
+  const int h8 = H & ~7;  // rows start on 16 bytes
+  for (int c = lane * 8; c < h8; c += 256) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(x + c));
+    const uint4 b = __ldg(reinterpret_cast<const uint4*>(e + c));
+    const __half2* ha = reinterpret_cast<const __half2*>(&a);
+    const __half2* hb = reinterpret_cast<const __half2*>(&b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 u = __half22float2(ha[j]), v = __half22float2(hb[j]);
+      s = fmaf(u.x, v.x, fmaf(u.y, v.y, s));
+    }
+  }
+  if (h8 + lane < H) s = fmaf(__half2float(x[h8 + lane]), __half2float(e[h8 + lane]), s);
+  return warp_sum(s);
+}
+
 constexpr int kRows = 32;   // rows per CTA of the forward's finishing kernel: one per lane
 constexpr int kWarps = 32;  // its warps share the slots
 
 // Joins the slots' (max, sum) pairs of 32 rows: warp w takes slots w, w + 32,
-// ...; lanes are rows, so every load is 256 contiguous bytes.
+// ...; lanes are rows, so every load is 256 contiguous bytes.  Before that,
+// while the GEMM still runs, warp w forms row w's target logit (x, E and the
+// targets are complete before the GEMM starts); it also replaces the GEMM's
+// value in the sum.
 __global__ void __launch_bounds__(kRows* kWarps)
     logprob_finish_kernel(const float2* __restrict__ part, const float* __restrict__ tgt_logit,
-                          const int* __restrict__ targets, int M, int V, int slots, float* __restrict__ logp,
+                          const int* __restrict__ targets, const __half* __restrict__ x, const __half* __restrict__ E,
+                          int M, int H, int V, int ldx, int lde, int slots, float* __restrict__ logp,
                           float* __restrict__ lse) {
   pdl_trigger();
-  pdl_wait();
   __shared__ float2 red[kWarps][kRows];
+  __shared__ float exact[kRows];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  {
+    const int row = blockIdx.x * kRows + w;
+    const int t = row < M ? targets[row] : -1;
+    if (t >= 0 && t < V) {
+      const float l = target_logit(x + static_cast<size_t>(row) * ldx, E + static_cast<size_t>(t) * lde, H, lane);
+      if (lane == 0) exact[w] = l;
+    }
+  }
+  pdl_wait();
   const int m = blockIdx.x * kRows + lane;
   float mx = -INFINITY, s = 0.f;
   auto join = [&](float2 o) {
@@ -52,10 +88,15 @@ __global__ void __launch_bounds__(kRows* kWarps)
     mx = -INFINITY;
     s = 0.f;
     for (int i = 0; i < kWarps; ++i) join(red[i][lane]);
-    const float l = mx + logf(s);
     const int t = targets[m];
+    const bool ok = t >= 0 && t < V;
+    if (ok) {
+      const float rough = tgt_logit[m], d = exact[lane] - rough;
+      if (isfinite(d)) s = fmaf(exp2f((rough - mx) * kLog2e), expm1f(d), s);
+    }
+    const float l = mx + logf(s);
     lse[m] = l;
-    logp[m] = t >= 0 && t < V ? tgt_logit[m] - l : 0.f;
+    logp[m] = ok ? exact[lane] - l : 0.f;
   }
 }
 
@@ -63,17 +104,23 @@ __global__ void __launch_bounds__(kRows* kWarps)
 // of acc), in slice order, and the target's own term in fp32.
 __global__ void __launch_bounds__(256)
     logprob_dx_kernel(const float* __restrict__ acc, int slabs, int slab_rows, int ld_acc,
-                      const __half* __restrict__ E, int lde, const float* __restrict__ tgt_logit,
+                      const __half* __restrict__ x, int ldx, const __half* __restrict__ E, int lde,
                       const float* __restrict__ lse, const float* __restrict__ dlogp, const int* __restrict__ targets,
                       int H, int V, float scale, __half* __restrict__ dx, int lddx) {
   pdl_trigger();
-  pdl_wait();
+  __shared__ float s_exact;
   const int m = blockIdx.x;
   const int t = targets[m];
   const bool ok = t >= 0 && t < V;
+  if (ok && threadIdx.x < 32) {  // inputs alone: while the last GEMM still runs
+    const float l = target_logit(x + static_cast<size_t>(m) * ldx, E + static_cast<size_t>(t) * lde, H, threadIdx.x);
+    if (threadIdx.x == 0) s_exact = l;
+  }
+  __syncthreads();
+  pdl_wait();
   // 1 - p_t without cancellation for a confident token
   const float g = ok ? scale * dlogp[m] : 0.f;
-  const float one_minus = ok ? -expm1f(tgt_logit[m] - lse[m]) : 0.f;
+  const float one_minus = ok ? -expm1f(s_exact - lse[m]) : 0.f;
   const float unshift = exp2f(-kProbShift);
   const __half* et = E + static_cast<size_t>(ok ? t : 0) * lde;
   const float* a0 = acc + static_cast<size_t>(m) * ld_acc;
@@ -110,30 +157,40 @@ __global__ void __launch_bounds__(256)
 
 // The backward's split of the vocabulary.
 struct BwdPlan {
-  int vc;         // columns per chunk (a multiple of 64 * ksplit, or all of V)
+  int vc;         // columns per chunk: a multiple of 1024, or all of V
   int ksplit;     // K slices asked of each chunk's dx GEMM
   int slabs;      // slices the widest chunk really has
   int slab_rows;  // rows of one slice's partial sums
   int ld_acc;
 };
 
-constexpr size_t kChunkElems = static_cast<size_t>(64) << 20;  // 128 MiB of fp16 probabilities
-constexpr int kMaxChunk = 16384;
+// 128 MiB of fp16 probabilities a chunk, as for the training step's head
+// (16384 columns at 4096 rows).  Few rows take the whole vocabulary at once:
+// 130 rows in 16384-column chunks, whose rows of E the second product would
+// find in L2, ran 525 us against 294 in one chunk.
+constexpr size_t kChunkElems = static_cast<size_t>(64) << 20;
 
 BwdPlan bwd_plan(int M, int H, int V) {
   BwdPlan p;
   p.ld_acc = (H + 3) / 4 * 4;
   p.slab_rows = (M + 255) / 256 * 256;
-  // as for the training step's head: 128 MiB of chunk values; at few rows the
-  // chunk's rows of E bound it instead (64 MiB at 2048 columns), so that the
-  // second product finds them in L2
-  const size_t fit = std::min<size_t>(kMaxChunk, kChunkElems / static_cast<size_t>(M));
-  p.vc = static_cast<int>(std::max<size_t>(1024, fit / 1024 * 1024));
-  // about four waves of tiles in the dx GEMM, or one at few rows
-  const int tiles = (M > 128 ? (M + 255) / 256 * 2 : 1) * ((H + 255) / 256);
-  p.ksplit = 4;
-  while (p.ksplit < 16 && tiles * p.ksplit * 2 <= gemm_num_sms()) p.ksplit *= 2;
+  const size_t fit = std::max<size_t>(1024, kChunkElems / static_cast<size_t>(M) / 1024 * 1024);
+  p.vc = static_cast<int>(std::min<size_t>(fit, (static_cast<size_t>(V) + 1023) / 1024 * 1024));
+  // K slices of the dx GEMM: the count whose waves of tiles waste least (74
+  // CTA pairs, or 148 CTAs up to 128 rows), each slice adding a little for its
+  // partial sums
+  const int tiles = (M > 128 ? (M + 255) / 256 : 1) * ((H + 255) / 256);
+  const int slots = std::max(1, M > 128 ? gemm_num_sms() / 2 : gemm_num_sms());
   const int nk = (std::min(p.vc, V) + 63) / 64;
+  double best = 1e30;
+  p.ksplit = 1;
+  for (int k = 1; k <= 32 && 4 * k <= std::max(4, nk); ++k) {
+    const double cost = static_cast<double>((tiles * static_cast<int64_t>(k) + slots - 1) / slots) / k * (1 + 0.004 * k);
+    if (cost < best) {
+      best = cost;
+      p.ksplit = k;
+    }
+  }
   const int per = (nk + p.ksplit - 1) / p.ksplit;
   p.slabs = (nk + per - 1) / per;
   return p;
@@ -149,10 +206,9 @@ struct PdlScope {  // the chain's kernels await one another (pdl_wait); the firs
 }  // namespace
 
 size_t lm_logprobs_workspace(int M, int H, int V, bool backward) {
-  const size_t tgt = up256(sizeof(float) * M);
-  if (!backward) return tgt + up256(sizeof(float2) * static_cast<size_t>(M) * ((V + 127) / 128));
+  if (!backward) return up256(sizeof(float) * M) + up256(sizeof(float2) * static_cast<size_t>(M) * ((V + 127) / 128));
   const BwdPlan p = bwd_plan(M, H, V);
-  return tgt + up256(sizeof(__half) * static_cast<size_t>(M) * p.vc) +
+  return up256(sizeof(__half) * static_cast<size_t>(M) * p.vc) +
          up256(sizeof(float) * static_cast<size_t>(p.slabs) * p.slab_rows * p.ld_acc);
 }
 
@@ -170,7 +226,7 @@ cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, fl
   if (e != cudaSuccess) return e;
   set_pdl(true);
   return launch_pdl(logprob_finish_kernel, (M + kRows - 1) / kRows, kRows * kWarps, 0, st, ea.part2, ea.tgt_logit,
-                    targets, M, V, slots, logp, lse);
+                    targets, x, E, M, H, V, ldx, lde, slots, logp, lse);
 }
 
 cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* targets, const float* lse,
@@ -178,9 +234,8 @@ cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* ta
                                  float scale, void* ws, int* err, cudaStream_t st) {
   const BwdPlan p = bwd_plan(M, H, V);
   char* w = static_cast<char*>(ws);
-  float* tgt_logit = reinterpret_cast<float*>(w);
-  __half* pc = reinterpret_cast<__half*>(w + up256(sizeof(float) * M));
-  float* acc = reinterpret_cast<float*>(w + up256(sizeof(float) * M) + up256(sizeof(__half) * static_cast<size_t>(M) * p.vc));
+  __half* pc = reinterpret_cast<__half*>(w);
+  float* acc = reinterpret_cast<float*>(w + up256(sizeof(__half) * static_cast<size_t>(M) * p.vc));
   PdlScope scope;
   set_pdl(false);
   for (int v0 = 0; v0 < V; v0 += p.vc) {
@@ -189,7 +244,6 @@ cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* ta
     EpiArgs ea;
     ea.targets = targets;
     ea.lse = lse;
-    ea.tgt_logit = tgt_logit;
     ea.vocab_off = v0;
     ea.out = pc;
     ea.ld_out = p.vc;
@@ -206,8 +260,8 @@ cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* ta
     e = gemm(Operand{pc, M, n, p.vc}, Operand{Ec, H, n, lde, true}, M, H, Epi::kStoreF32, eb, err, st, 256);
     if (e != cudaSuccess) return e;
   }
-  return launch_pdl(logprob_dx_kernel, M, 256, 0, st, acc, p.slabs, p.slab_rows, p.ld_acc, E, lde, tgt_logit, lse, dlogp,
-                    targets, H, V, scale, dx, lddx);
+  return launch_pdl(logprob_dx_kernel, M, 256, 0, st, acc, p.slabs, p.slab_rows, p.ld_acc, x, ldx, E, lde, lse,
+                    dlogp, targets, H, V, scale, dx, lddx);
 }
 
 }  // namespace llmcu

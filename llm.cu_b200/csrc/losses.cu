@@ -12,6 +12,7 @@
 // of their row, or buffers that are not aligned, are taken element by element.
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "common.cuh"
 
@@ -20,6 +21,7 @@ namespace llmcu {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMainBlocks = 4;  // resident CTAs of the policy loss's main kernel on an SM
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
@@ -27,14 +29,56 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
-// Sum over the CTA, in a fixed order, for every thread; `red` holds 32 values.
-__device__ __forceinline__ double block_sum(double v, double* red) {
-  v = warp_sum_f64(v);
+// Sums of N values over the CTA, in a fixed order, for every thread; `red`
+// holds N * 32 values.
+template <int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double* red) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = warp_sum_f64(v[k]);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if (lane == 0) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) red[k * 32 + w] = v[k];
+  }
   __syncthreads();
-  const int n = blockDim.x >> 5;
-  return warp_sum_f64((threadIdx.x & 31) < n ? red[threadIdx.x & 31] : 0.0);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] = 0.0;
+    for (int i = 0; i < nw; ++i) v[k] += red[k * 32 + i];
+  }
+}
+// The CTAs' sums of a cluster, in rank order.  Each CTA stores its own into
+// every other's shared memory (`slots`, 8 * N values), so that after one
+// cluster barrier all reads are local and a CTA may leave at any time.  The
+// kernel has arrived at the cluster barrier once before (cluster_begin), which
+// this waits for: a CTA's shared memory exists once it runs.  `all` false:
+// rank 0 alone gets the sums, and the others do not wait.
+constexpr int kMaxCluster = 8;
+__device__ __forceinline__ void cluster_begin(int C) {
+  if (C > 1) cluster_arrive();
+}
+template <int N>
+__device__ __forceinline__ void cluster_sums(double (&v)[N], double* slots, int C, int rank, bool first,
+                                             bool all = true) {
+  if (C == 1) return;
+  if (first) cluster_wait();
+  const int t = threadIdx.x;
+  const int c = t / N, k = t - c * N;
+  if (c < (all ? C : 1)) {
+    double mine = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) mine = k == i ? v[i] : mine;
+    st_cluster_f64(mapa_shared(smem_u32(slots + rank * N + k), c), mine);
+  }
+  cluster_arrive();
+  if (!all && rank != 0) return;
+  cluster_wait();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0.0;
+    for (int r = 0; r < C; ++r) v[i] += slots[r * N + i];
+  }
 }
 
 // One row of a [rows, ld] buffer in quads.
@@ -113,13 +157,14 @@ constexpr int kKept = 8;  // quads of each row whose mask bits a thread keeps
 
 __global__ void __launch_bounds__(kThreads)
     preference_kernel(PreferenceArgs a) {
-  __shared__ double red[32];
-  __shared__ double part[4];
+  __shared__ double red[4 * 32];
+  __shared__ double slots[4 * kMaxCluster];
   const int C = a.cluster;
-  const uint32_t rank = C > 1 ? cluster_ctarank() : 0u;
+  const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  cluster_begin(C);
   const int pair = blockIdx.x / C;
   const int stride = C * kThreads;
-  const int t0 = static_cast<int>(rank) * kThreads + threadIdx.x;
+  const int t0 = rank * kThreads + threadIdx.x;
   double sum[2] = {0.0, 0.0};
   int cnt[2] = {0, 0};
   uint64_t kept = 0;
@@ -145,22 +190,20 @@ __global__ void __launch_bounds__(kThreads)
       cnt[side] += __popc(bits);
     }
   }
-  double v[4] = {sum[0], sum[1], static_cast<double>(cnt[0]), static_cast<double>(cnt[1])};
-  const int nv = a.mean_tokens ? 4 : 2;
-  for (int k = 0; k < nv; ++k) v[k] = block_sum(v[k], red);
-  if (C > 1) {
-    if (threadIdx.x == 0)
-      for (int k = 0; k < nv; ++k) part[k] = v[k];
-    cluster_sync_all();
-    const uint32_t mine = smem_u32(part);
-    for (int k = 0; k < nv; ++k) {
-      v[k] = 0.0;
-      for (int c = 0; c < C; ++c) v[k] += ld_cluster_f64(mapa_shared(mine + 8 * k, c));
-    }
-    cluster_sync_all();  // nobody leaves while its sums are read
+  double share[2] = {1.0, 1.0};
+  if (a.mean_tokens) {
+    double v[4] = {sum[0], sum[1], static_cast<double>(cnt[0]), static_cast<double>(cnt[1])};
+    block_sums(v, red);
+    cluster_sums(v, slots, C, rank, true);
+    sum[0] = v[0];
+    sum[1] = v[1];
+    share[0] = 1.0 / fmax(v[2], 1.0);
+    share[1] = 1.0 / fmax(v[3], 1.0);
+  } else {
+    block_sums(sum, red);
+    cluster_sums(sum, slots, C, rank, true);
   }
-  const double share[2] = {a.mean_tokens ? 1.0 / fmax(v[2], 1.0) : 1.0, a.mean_tokens ? 1.0 / fmax(v[3], 1.0) : 1.0};
-  const double R[2] = {v[0] * share[0], v[1] * share[1]};
+  const double R[2] = {sum[0] * share[0], sum[1] * share[1]};
   const double beta = a.beta, D = R[0] - R[1];
   float loss, dD;
   if (a.kind == kPrefSquared) {
@@ -188,10 +231,9 @@ __global__ void __launch_bounds__(kThreads)
       a.reward[a.pairs + pair] = static_cast<float>(beta * R[1]);
     }
   }
-  if (!a.dlogp) return;
   const float up = a.dloss ? __ldg(a.dloss + pair) : 1.0f / static_cast<float>(a.pairs);
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
+  for (int side = 0; side < 2 && a.dlogp; ++side) {
     const RowSpan r(static_cast<int64_t>(side) * a.pairs + pair, a.ld, a.seq);
     const float g = (side ? -dD : dD) * up * static_cast<float>(share[side]);
     int k = 0;
@@ -216,19 +258,170 @@ __global__ void __launch_bounds__(kThreads)
 // The loss is the sum of l times its row's weight: 1 / (scored tokens), 1 /
 // (rows * the row's scored tokens), or 1 / norm.
 //
-// Whether a token clips is decided on delta in 64 bits against the logarithm
-// of the border, so that a token next to it falls on the side that the inputs
-// say.  e^d - d - 1 loses everything to cancellation for a small d; below 1/2
-// its series d^2/2 (1 + d/3 (1 + d/4 (...))) is summed instead (ten terms: the
-// next is under 2^-24 of the sum).
-__device__ __forceinline__ float kl_of(float d, float em1) {
-  if (fabsf(d) < 0.5f) {
-    float s = 1.f;
-#pragma unroll
-    for (int k = 10; k >= 3; --k) s = fmaf(s, d * (1.0f / static_cast<float>(k)), 1.f);
-    return 0.5f * d * d * s;
+// Whether a token clips is decided on delta against the logarithm of the
+// border; next to it (which fp32 cannot tell) in 64 bits, so that the token
+// falls on the side that the inputs say.
+//
+// e^d - d - 1 loses everything to cancellation for a small d; below 1 its
+// series d^2 (1/2! + d/3! + ...) is summed instead, to d^12 / 12! (the next
+// term is under 2^-25 of the sum), and e^d - 1 is d more.
+struct PolicyToken {
+  float loss, kl, grad;
+  bool clip;
+};
+__device__ __forceinline__ PolicyToken policy_token(const PolicyArgs& a, float lp, float old, float A, float ref) {
+  PolicyToken t;
+  const float delta = lp - old;
+  const float rA = expf(delta) * A;
+  // clips above hi and below lo
+  const bool pos = A > 0.f;
+  const float hi = pos ? a.f_high : a.f_dual, lo = pos ? -INFINITY : a.f_low;
+  bool above = delta > hi, below = delta < lo;
+  if (fminf(fabsf(delta - hi), fabsf(delta - lo)) < a.near) {
+    const double d64 = static_cast<double>(lp) - static_cast<double>(old);
+    above = d64 > (pos ? a.log_high : a.log_dual);
+    below = !pos && d64 < a.log_low;
   }
-  return em1 - d;
+  t.clip = (above || below) && (pos || A < 0.f);
+  const float bound = below ? a.low : pos ? a.high : a.dual;
+  t.loss = t.clip ? -bound * A : -rA;
+  t.grad = t.clip ? 0.f : -rA;
+  t.kl = 0.f;
+  if (a.ref) {
+    const float d = ref - lp;
+    float s = 1.f / 479001600.f;
+    s = fmaf(s, d, 1.f / 39916800.f);
+    s = fmaf(s, d, 1.f / 3628800.f);
+    s = fmaf(s, d, 1.f / 362880.f);
+    s = fmaf(s, d, 1.f / 40320.f);
+    s = fmaf(s, d, 1.f / 5040.f);
+    s = fmaf(s, d, 1.f / 720.f);
+    s = fmaf(s, d, 1.f / 120.f);
+    s = fmaf(s, d, 1.f / 24.f);
+    s = fmaf(s, d, 1.f / 6.f);
+    s = fmaf(s, d, 0.5f);
+    t.kl = d * d * s;
+    float em1 = d + t.kl;
+    if (!(fabsf(d) < 1.f)) {
+      em1 = expf(d) - 1.f;
+      t.kl = em1 - d;
+    }
+    t.grad = fmaf(-a.beta, em1, t.grad);
+    t.loss = fmaf(a.beta, t.kl, t.loss);
+  }
+  return t;
+}
+
+// The four tokens of a quad: gradients (0 where nothing is scored), sums.
+struct PolicyQuad {
+  float lp[4], old[4], adv[4], ref[4];
+  __device__ __forceinline__ void load(const PolicyArgs& a, int row, int64_t i, int64_t first, int64_t end) {
+    load4(a.logp, i, first, end, a.vec, 0.f, lp);
+    load4(a.old, i, first, end, a.vec, 0.f, old);
+    if (a.token_adv) {
+      load4(a.adv, i, first, end, a.vec, 0.f, adv);
+    } else {
+      adv[0] = adv[1] = adv[2] = adv[3] = __ldg(a.adv + row);
+    }
+    if (a.ref) load4(a.ref, i, first, end, a.vec, 0.f, ref);
+  }
+  __device__ __forceinline__ void run(const PolicyArgs& a, uint32_t bits, float weight, float (&g)[4], float& loss,
+                                      float& kl, int& clips) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const PolicyToken t = policy_token(a, lp[j], old[j], adv[j], ref[j]);
+      const bool on = (bits >> j) & 1;
+      g[j] = on ? t.grad * weight : 0.f;
+      loss += on ? t.loss : 0.f;
+      kl += on ? t.kl : 0.f;
+      clips += on && t.clip;
+    }
+  }
+};
+
+// Row, first element and row's ends of unit u.
+struct PolicyUnit {
+  int row;
+  bool any;  // the unit holds tokens of its row
+  int64_t i, first, end;
+  __device__ __forceinline__ PolicyUnit(const PolicyArgs& a, int64_t u) {
+    row = static_cast<int>(__umulhi(static_cast<uint32_t>(u), a.div_m) >> a.div_s);
+    const int q = static_cast<int>(u) - row * a.row_quads;
+    first = static_cast<int64_t>(row) * a.ld;
+    end = first + a.seq;
+    i = (first & ~int64_t{3}) + 4 * q;
+    any = u < a.units && i < end;
+  }
+  __device__ __forceinline__ uint32_t mask(const PolicyArgs& a) const {
+    return any ? load_mask(a.mask, i, first, end, a.vec) : 0u;
+  }
+};
+
+__device__ __forceinline__ void write_stats(const double (&v)[4], float* stats) {
+  const double t = fmax(v[3], 1.0);
+  stats[0] = static_cast<float>(v[0]);
+  stats[1] = static_cast<float>(v[1] / t);
+  stats[2] = static_cast<float>(v[2] / t);
+  stats[3] = static_cast<float>(v[3]);
+}
+
+// Everything in one launch, for batches of at most kSmallUnits quads: each
+// thread of one cluster holds one quad, the scored tokens are counted (of each
+// row in shared memory, for means over rows), and the counts and then the sums
+// meet over distributed shared memory.
+constexpr int kSmallCluster = kMaxCluster;
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallUnits = kSmallCluster * kSmallThreads;
+constexpr int kSmallRows = 1024;
+
+__global__ void __launch_bounds__(kSmallThreads) policy_small_kernel(PolicyArgs a, int C) {
+  __shared__ double red[4 * 32];
+  __shared__ double slots[2][4 * kMaxCluster];
+  __shared__ int rows[kSmallRows];  // this CTA's scored tokens of each row
+  extern __shared__ int all_rows[];  // [C][batch]: every CTA's
+  const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  cluster_begin(C);
+  const bool by_row = a.agg == kPolicySequenceMean;
+  const int nt = blockDim.x;
+  if (by_row) {
+    for (int r = threadIdx.x; r < a.batch; r += nt) rows[r] = 0;
+    __syncthreads();
+  }
+  const PolicyUnit p(a, rank * nt + threadIdx.x);
+  const uint32_t bits = p.mask(a);
+  PolicyQuad quad;
+  if (p.any) quad.load(a, p.row, p.i, p.first, p.end);
+  if (by_row && bits) atomicAdd(&rows[p.row], __popc(bits));
+  float weight = a.inv_norm;
+  if (a.agg == kPolicyTokenMean) {
+    double n[1] = {static_cast<double>(__popc(bits))};
+    block_sums(n, red);
+    cluster_sums(n, slots[0], C, rank, true);
+    weight = static_cast<float>(1.0 / fmax(n[0], 1.0));
+  } else if (by_row) {
+    if (C > 1) cluster_wait();
+    __syncthreads();
+    const uint32_t to = smem_u32(all_rows + rank * a.batch);
+    for (int e = threadIdx.x; e < a.batch * C; e += nt) {
+      const int c = e / a.batch, r = e - c * a.batch;
+      st_cluster_s32(mapa_shared(to + 4 * r, c), rows[r]);
+    }
+    cluster_sync_all();
+    if (bits) {
+      int n = 0;
+      for (int c = 0; c < C; ++c) n += all_rows[c * a.batch + p.row];
+      weight = 1.0f / (static_cast<float>(n) * static_cast<float>(a.batch));
+    }
+  }
+  float g[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, kl = 0.f;
+  int clips = 0;
+  if (bits) quad.run(a, bits, weight, g, l, kl, clips);
+  if (a.dlogp && p.any) store4(a.dlogp, p.i, p.first, p.end, a.vec, g);
+  double v[4] = {static_cast<double>(l * weight), static_cast<double>(kl), static_cast<double>(clips),
+                 static_cast<double>(__popc(bits))};
+  block_sums(v, red);
+  cluster_sums(v, slots[1], C, rank, a.agg == kPolicyConstant, false);
+  if (rank == 0 && threadIdx.x == 0) write_stats(v, a.stats);
 }
 
 // Scored tokens: of each row (one CTA or warp a row) into counts[row], or of
@@ -255,10 +448,8 @@ __global__ void __launch_bounds__(kThreads) policy_count_kernel(PolicyArgs a, in
   } else {
     for (int64_t u = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; u < a.units;
          u += static_cast<int64_t>(gridDim.x) * kThreads) {
-      const int row = static_cast<int>(__umulhi(static_cast<uint32_t>(u), a.div_m) >> a.div_s);
-      const RowSpan r(row, a.ld, a.seq);
-      const int q = static_cast<int>(u) - row * a.row_quads;
-      if (q < r.nq) n += __popc(load_mask(a.mask, (r.q0 + q) << 2, r.first, r.end, a.vec));
+      const PolicyUnit p(a, u);
+      n += __popc(p.mask(a));
     }
   }
   n = __reduce_add_sync(0xffffffffu, n);
@@ -270,81 +461,53 @@ __global__ void __launch_bounds__(kThreads) policy_count_kernel(PolicyArgs a, in
   }
 }
 
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kMainBlocks)
     policy_main_kernel(PolicyArgs a, const int* __restrict__ counts, int n_counts, double* __restrict__ partial) {
   pdl_trigger();
   pdl_wait();
-  __shared__ double red[32];
+  __shared__ double red[4 * 32];
   float weight = a.inv_norm;
   if (a.agg == kPolicyTokenMean) {
-    double n = 0.0;
-    for (int i = threadIdx.x; i < n_counts; i += kThreads) n += static_cast<double>(counts[i]);
-    n = block_sum(n, red);
-    weight = static_cast<float>(1.0 / fmax(n, 1.0));
+    double n[1] = {0.0};
+    for (int i = threadIdx.x; i < n_counts; i += kThreads) n[0] += static_cast<double>(counts[i]);
+    block_sums(n, red);
+    weight = static_cast<float>(1.0 / fmax(n[0], 1.0));
   }
-  double s_loss = 0.0, s_kl = 0.0;
-  int64_t clips = 0, tokens = 0;
-  for (int64_t u = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; u < a.units;
-       u += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int row = static_cast<int>(__umulhi(static_cast<uint32_t>(u), a.div_m) >> a.div_s);
-    const RowSpan r(row, a.ld, a.seq);
-    const int q = static_cast<int>(u) - row * a.row_quads;
-    if (q >= r.nq) continue;
-    const int64_t i = (r.q0 + q) << 2;
-    const uint32_t bits = load_mask(a.mask, i, r.first, r.end, a.vec);
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+  int clips = 0;
+  int64_t tokens = 0;
+  // the mask of the next unit is fetched a turn ahead, so that the loads it
+  // decides on wait for nothing
+  // a CTA takes a run of units
+  const int64_t run = (a.units + gridDim.x - 1) / gridDim.x;
+  const int64_t u_end = min(a.units, (blockIdx.x + 1) * run);
+  int64_t u = blockIdx.x * run + threadIdx.x;
+  PolicyUnit next(a, min(u, u_end));
+  uint32_t next_bits = u < u_end ? next.mask(a) : 0u;
+  for (; u < u_end; u += kThreads) {
+    const PolicyUnit p = next;
+    const uint32_t bits = next_bits;
     float g[4] = {0.f, 0.f, 0.f, 0.f};
+    PolicyQuad quad;
+    if (bits) quad.load(a, p.row, p.i, p.first, p.end);
+    if (u + kThreads < u_end) {
+      next = PolicyUnit(a, u + kThreads);
+      next_bits = next.mask(a);
+    }
     if (bits) {
-      if (a.agg == kPolicySequenceMean) weight = 1.0f / (static_cast<float>(counts[row]) * static_cast<float>(a.batch));
-      float lp[4], old[4], adv[4], ref[4];
-      load4(a.logp, i, r.first, r.end, a.vec, 0.f, lp);
-      load4(a.old, i, r.first, r.end, a.vec, 0.f, old);
-      if (a.token_adv) {
-        load4(a.adv, i, r.first, r.end, a.vec, 0.f, adv);
-      } else {
-        adv[0] = adv[1] = adv[2] = adv[3] = __ldg(a.adv + row);
-      }
-      if (a.ref) load4(a.ref, i, r.first, r.end, a.vec, 0.f, ref);
+      if (a.agg == kPolicySequenceMean)
+        weight = 1.0f / (static_cast<float>(counts[p.row]) * static_cast<float>(a.batch));
       float l = 0.f, kl = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!((bits >> j) & 1)) continue;
-        const double delta = static_cast<double>(lp[j]) - static_cast<double>(old[j]);
-        const float A = adv[j];
-        const float rA = expf(static_cast<float>(delta)) * A;
-        float obj = rA;
-        bool clip = false;
-        if (A > 0.f && delta > a.log_high) {
-          obj = a.high * A;
-          clip = true;
-        } else if (A < 0.f && delta < a.log_low) {
-          obj = a.low * A;
-          clip = true;
-        } else if (A < 0.f && delta > a.log_dual) {
-          obj = a.dual * A;
-          clip = true;
-        }
-        float gr = clip ? 0.f : -rA;
-        float lj = -obj;
-        if (a.ref) {
-          const float d = ref[j] - lp[j];
-          const float em1 = expm1f(d);
-          const float k3 = kl_of(d, em1);
-          gr = fmaf(-a.beta, em1, gr);
-          lj = fmaf(a.beta, k3, lj);
-          kl += k3;
-        }
-        l += lj;
-        clips += clip;
-        g[j] = gr * weight;
-      }
-      s_loss += static_cast<double>(l) * static_cast<double>(weight);
-      s_kl += static_cast<double>(kl);
+      quad.run(a, bits, weight, g, l, kl, clips);
+      v[0] += static_cast<double>(l * weight);
+      v[1] += static_cast<double>(kl);
       tokens += __popc(bits);
     }
-    if (a.dlogp) store4(a.dlogp, i, r.first, r.end, a.vec, g);
+    if (a.dlogp && p.any) store4(a.dlogp, p.i, p.first, p.end, a.vec, g);
   }
-  const double v[4] = {block_sum(s_loss, red), block_sum(s_kl, red), block_sum(static_cast<double>(clips), red),
-                       block_sum(static_cast<double>(tokens), red)};
+  v[2] = static_cast<double>(clips);
+  v[3] = static_cast<double>(tokens);
+  block_sums(v, red);
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) partial[blockIdx.x * 4 + k] = v[k];
@@ -356,20 +519,13 @@ __global__ void __launch_bounds__(kThreads) policy_stats_kernel(const double* __
                                                                float* __restrict__ stats) {
   pdl_trigger();
   pdl_wait();
-  __shared__ double red[32];
+  __shared__ double red[4 * 32];
   double v[4] = {0.0, 0.0, 0.0, 0.0};
   for (int i = threadIdx.x; i < n; i += kThreads)
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] += partial[i * 4 + k];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = block_sum(v[k], red);
-  if (threadIdx.x == 0) {
-    const double t = fmax(v[3], 1.0);
-    stats[0] = static_cast<float>(v[0]);
-    stats[1] = static_cast<float>(v[1] / t);
-    stats[2] = static_cast<float>(v[2] / t);
-    stats[3] = static_cast<float>(v[3]);
-  }
+  block_sums(v, red);
+  if (threadIdx.x == 0) write_stats(v, stats);
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -378,35 +534,24 @@ constexpr int kCountBlocks = 296;  // CTAs of the token count: two an SM
 
 int policy_blocks(int64_t units) {
   const int64_t want = (units + kThreads - 1) / kThreads;
-  return static_cast<int>(std::min<int64_t>(want, 8 * static_cast<int64_t>(gemm_num_sms())));
+  return static_cast<int>(std::min<int64_t>(want, kMainBlocks * static_cast<int64_t>(gemm_num_sms())));
 }
 
 }  // namespace
 
 cudaError_t preference_loss(PreferenceArgs a, cudaStream_t st) {
   a.vec = aligned(a.logp, 16) && aligned(a.ref, 16) && aligned(a.mask, 4) && aligned(a.dlogp, 16);
-  // CTAs a pair: enough that a thread meets at most about two quads of each
+  // CTAs a pair: enough that a thread meets at most about four quads of each
   // row, but no more than keep the GPU's resident CTAs (8 an SM) busy
   int C = 1;
   const int quads = a.seq / 4 + 2;
-  while (C < 8 && quads > 2 * C * kThreads && static_cast<int64_t>(a.pairs) * C < 8LL * gemm_num_sms()) C *= 2;
+  while (C < 8 && quads > 4 * C * kThreads && static_cast<int64_t>(a.pairs) * C < 8LL * gemm_num_sms()) C *= 2;
   a.cluster = C;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.pairs) * C);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = C > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, preference_kernel, a);
+  return launch_cluster(preference_kernel, static_cast<unsigned>(a.pairs) * C, kThreads, C, 0, st, a);
 }
 
 size_t policy_loss_workspace(int batch) {
-  const size_t partial = sizeof(double) * 4 * 8 * static_cast<size_t>(gemm_num_sms());
+  const size_t partial = sizeof(double) * 4 * kMainBlocks * static_cast<size_t>(gemm_num_sms());
   return partial + sizeof(int) * std::max<size_t>(kCountBlocks, static_cast<size_t>(batch));
 }
 
@@ -424,8 +569,24 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
   while ((2ull << s) < d) ++s;
   a.div_s = s;
   a.div_m = static_cast<uint32_t>(((1ull << (32 + s)) + d - 1) / d);
+  a.f_low = static_cast<float>(a.log_low);
+  a.f_high = static_cast<float>(a.log_high);
+  a.f_dual = static_cast<float>(a.log_dual);
+  // how near to a border fp32 cannot be trusted: some steps of the largest
+  double most = 1.0;
+  for (double b : {a.log_low, a.log_high, a.log_dual})
+    if (std::isfinite(b)) most = std::max(most, std::fabs(b));
+  a.near = static_cast<float>(1e-6 * most);
+  if (a.units <= kSmallUnits && (a.agg != kPolicySequenceMean || a.batch <= kSmallRows)) {
+    // CTAs of 256 threads, of 1024 once a cluster of eight does not suffice
+    const int nt = a.units <= kSmallCluster * kThreads ? kThreads : kSmallThreads;
+    int C = 1;
+    while (C * nt < a.units) C *= 2;
+    const size_t smem = a.agg == kPolicySequenceMean ? sizeof(int) * C * a.batch : 0;
+    return launch_cluster(policy_small_kernel, C, nt, C, smem, st, a, C);
+  }
   double* partial = static_cast<double*>(ws);
-  int* counts = reinterpret_cast<int*>(partial + 4 * 8 * static_cast<size_t>(gemm_num_sms()));
+  int* counts = reinterpret_cast<int*>(partial + 4 * kMainBlocks * static_cast<size_t>(gemm_num_sms()));
   const bool was = pdl_enabled();
   set_pdl(false);
   cudaError_t e = cudaSuccess;
