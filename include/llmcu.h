@@ -510,6 +510,42 @@ typedef struct {
 llmcu_status llmcu_muon_update(const llmcu_muon_cfg* cfg, float* w, const float* grad, float* momentum, int count,
                                int rows, int cols, void* stream);
 
+/* The same on a training context: the step's forward, one of these losses in
+ * place of the cross-entropy, and the backward into the adapter gradients
+ * (llmcu_get_lora_grads; then llmcu_adamw or llmcu_muon).  tokens and targets
+ * are HOST int32 [batch, seq] as for llmcu_train_step, with its argument rules,
+ * but for the targets: one outside [0, vocab) marks a position that is not
+ * scored (prompt, padding), and positions are scored whatever
+ * llmcu_run_cfg.loss_all_positions says.  Log-probabilities are HOST fp32
+ * [batch, seq]; what they hold where nothing is scored is not used.  Data
+ * parallel: the gradients and the loss are averaged over ranks. */
+
+/* Log-probabilities of the targets (0 where not scored) under the current
+ * adapters (adapters = 1) or the base alone (0: the reference model of the
+ * losses below). */
+llmcu_status llmcu_score(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* targets, int batch, int seq,
+                         int adapters, float* logp);
+/* Mean paired preference loss of batch / 2 pairs: sequences 0 .. batch/2 - 1
+ * are the chosen ones, batch/2 .. batch - 1 the rejected ones.  ref_logp
+ * (nullable): llmcu_score's of the reference model.  rewards (nullable, host
+ * [batch]): beta * R of each sequence. */
+llmcu_status llmcu_preference_forward_backward(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* targets,
+                                               const float* ref_logp, int batch, int seq,
+                                               const llmcu_preference_cfg* cfg, float* loss_out, float* rewards);
+/* Clipped policy loss: old_logp is llmcu_score's at sampling time; ref_logp
+ * (nullable) the reference model's; advantages host fp32 [batch], or [batch,
+ * seq] with token_advantages.  stats (nullable, host, 4 floats) as for
+ * llmcu_policy_loss (this rank's). */
+llmcu_status llmcu_policy_forward_backward(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* targets,
+                                           const float* old_logp, const float* ref_logp, const float* advantages,
+                                           int batch, int seq, const llmcu_policy_cfg* cfg, float* loss_out,
+                                           float* stats);
+/* Muon update of every adapter matrix with the gradients in place, in one
+ * launch.  Its momentum lies where AdamW keeps its first moment (so
+ * llmcu_save_adamw_state / llmcu_load_adamw_state carry it, and
+ * llmcu_reset_optimizer clears it): do not mix the two without a reset. */
+llmcu_status llmcu_muon(llmcu_ctx* ctx, const llmcu_muon_cfg* cfg);
+
 #ifdef __cplusplus
 }
 #endif

@@ -262,10 +262,23 @@ cudaError_t ce_stream_rescale(__half* pc, int ldp, const float* part_ref, int sl
 // After the last chunk: lse and row losses (+ their sum at row_loss[M]) from
 // the slot partials; d_xf -> gscale * (exp(ref - lse) d_xf + (p_t - 1) E_t)
 // for rows in the loss, 0 for the others (src/kernels/loss.cu:62-69).
+// With row_w and norm (loss_norm's) the gradient is that of a loss given by
+// row_w[m] = dL/dlogp[m]: gscale is replaced by -row_w[m] * norm[0] * gscale,
+// and the row losses are not summed.
 cudaError_t ce_stream_finish(const float* part_ref, const float* part_sum, const float* tgt_logit, const float* ref,
                              const uint8_t* valid, const int* targets, const __half* E, int M, int H, int V,
                              int slots, float gscale, float* lse, float* row_loss_and_sum, float* d_xf,
-                             cudaStream_t st);
+                             cudaStream_t st, const float* row_w = nullptr, const float* norm = nullptr);
+// The rows' target log-probabilities after the last chunk (0 where the target
+// lies outside the vocabulary), as lm_logprobs gives them.
+cudaError_t ce_stream_logp(const float* part_ref, const float* part_sum, const float* tgt_logit, const int* targets,
+                           const __half* xf, const __half* E, int M, int H, int V, int slots, float* logp,
+                           cudaStream_t st);
+// mask[m] = 1 where targets[m] lies in the vocabulary
+cudaError_t scored_rows(uint8_t* mask, const int* targets, int M, int V, cudaStream_t st);
+// norm[0], norm[1]: a power of two that brings max |w| into [1/2, 1), and its
+// inverse; *total = sum of loss[0 .. n)
+cudaError_t loss_norm(const float* w, int M, const float* loss, int n, float* norm, float* total, cudaStream_t st);
 cudaError_t adamw_flat(float* p, const float* g, float* m, float* v, int64_t n, float lr, float b1, float b2,
                        float eps, float wd, float bc1, float bc2, float gscale, cudaStream_t st);
 cudaError_t fill_f32_2d(float* p, int ld, int rows, int cols, float v, cudaStream_t st);
@@ -287,6 +300,9 @@ cudaError_t dequant_rows_f16(const int8_t* q, const float* scale, int rows, int 
 // ---- logprobs.cu (x [M, H], E [V, H] fp16 with row strides ldx, lde; targets
 // outside [0, V) score nothing: logp 0, dx row 0)
 size_t lm_logprobs_workspace(int M, int H, int V, bool backward);
+// part: ceil(V / 128) * M pairs; tgt_logit: M floats
+cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, float* logp, float* lse, int M, int H,
+                        int V, int ldx, int lde, float2* part, float* tgt_logit, int* err, cudaStream_t st);
 cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, float* logp, float* lse, int M, int H,
                         int V, int ldx, int lde, void* ws, int* err, cudaStream_t st);
 cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* targets, const float* lse,

@@ -531,14 +531,17 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 // lse - l_target (src/kernels/loss.cu:66-67), and the logits' gradient
 // applied to E in fp32: d_xf held sum_{j != t} exp(l_j - ref) E_j, so
 // dX = exp(ref - lse) d_xf + (p_t - 1) E_t (src/kernels/loss.cu:62-69 times
-// E), scaled by gscale; 0 for rows outside the loss.  A block takes kRowWarps
-// rows: a warp reduces one row's partials, then the whole block updates the
-// rows' d_xf.
+// E), scaled by gscale; 0 for rows outside the loss.  With row_w (a loss other
+// than the mean cross-entropy, given by its gradient for each row's
+// log-probability) gscale becomes -row_w[m] * *norm * gscale.  A block takes
+// kRowWarps rows: a warp reduces one row's partials, then the whole block
+// updates the rows' d_xf.
 __global__ void __launch_bounds__(kRowWarps * 32)
     ce_stream_finish_kernel(const float* __restrict__ part_ref, const float* __restrict__ part_sum,
                             const float* __restrict__ tgt_logit, const float* __restrict__ ref,
                             const uint8_t* __restrict__ valid, const int* __restrict__ targets,
                             const __half* __restrict__ E, int M, int H, int V, int slots, float gscale,
+                            const float* __restrict__ row_w, const float* __restrict__ norm,
                             float* __restrict__ lse, float* __restrict__ row_loss, float* __restrict__ d_xf) {
   pdl_trigger();
   pdl_wait();
@@ -559,10 +562,11 @@ __global__ void __launch_bounds__(kRowWarps * 32)
     const float l = mx + logf(s);
     const bool ok = valid[m] != 0;
     if (lane == 0) {
+      const float gs = row_w ? -row_w[m] * *norm * gscale : gscale;
       lse[m] = l;
       row_loss[m] = ok ? l - tgt_logit[m] : 0.f;
-      s_a[w] = ok ? exp2f((ref[m] - l) * kLog2e) * gscale : 0.f;
-      s_pt1[w] = ok ? (exp2f((tgt_logit[m] - l) * kLog2e) - 1.0f) * gscale : 0.f;
+      s_a[w] = ok ? exp2f((ref[m] - l) * kLog2e) * gs : 0.f;
+      s_pt1[w] = ok ? (exp2f((tgt_logit[m] - l) * kLog2e) - 1.0f) * gs : 0.f;
       s_t[w] = min(max(targets[m], 0), V - 1);
       s_ok[w] = ok;
     }
@@ -590,6 +594,51 @@ __global__ void __launch_bounds__(kRowWarps * 32)
                        fmaf(a, v1.w, pt1 * e[7]));
       *reinterpret_cast<float4*>(dx + c0) = v0;
       *reinterpret_cast<float4*>(dx + c0 + 4) = v1;
+    }
+  }
+}
+
+// Mask of the rows whose target lies in the vocabulary (the others are not
+// scored: prompt and padding).
+__global__ void scored_rows_kernel(uint8_t* __restrict__ mask, const int* __restrict__ targets, int M, int V) {
+  pdl_trigger();
+  pdl_wait();
+  const int m = blockIdx.x * blockDim.x + threadIdx.x;
+  if (m < M) mask[m] = targets[m] >= 0 && targets[m] < V ? 1 : 0;
+}
+
+// One CTA: norm[0] = the power of two that brings the largest |w[m]| into
+// [1/2, 1) (1 where all are 0, or one is not finite), norm[1] = 1 / norm[0] --
+// the fp16 backward then carries gradients of the size it does for the
+// cross-entropy, whatever the loss's scale; *total = the sum of loss[0 .. n)
+// in a fixed order.
+__global__ void __launch_bounds__(1024) loss_norm_kernel(const float* __restrict__ w, int M,
+                                                         const float* __restrict__ loss, int n,
+                                                         float* __restrict__ norm, float* __restrict__ total) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float red[2][32];
+  float mx = 0.f, s = 0.f;
+  for (int i = threadIdx.x; i < M; i += blockDim.x) mx = fmaxf(mx, fabsf(w[i]));
+  for (int i = threadIdx.x; i < n; i += blockDim.x) s += loss[i];
+  mx = warp_max(mx);
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) {
+    red[0][threadIdx.x >> 5] = mx;
+    red[1][threadIdx.x >> 5] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const bool in = threadIdx.x < (blockDim.x >> 5);
+    mx = warp_max(in ? red[0][threadIdx.x] : 0.f);
+    s = warp_sum(in ? red[1][threadIdx.x] : 0.f);
+    if (threadIdx.x == 0) {
+      int e = 0;
+      if (mx > 0.f && isfinite(mx)) frexpf(mx, &e);
+      e = min(max(e, -100), 100);
+      norm[0] = ldexpf(1.f, -e);
+      norm[1] = ldexpf(1.f, e);
+      *total = s;
     }
   }
 }
@@ -952,13 +1001,23 @@ cudaError_t ce_stream_rescale(__half* pc, int ldp, const float* part_ref, int sl
 cudaError_t ce_stream_finish(const float* part_ref, const float* part_sum, const float* tgt_logit, const float* ref,
                              const uint8_t* valid, const int* targets, const __half* E, int M, int H, int V,
                              int slots, float gscale, float* lse, float* row_loss_and_sum, float* d_xf,
-                             cudaStream_t st) {
+                             cudaStream_t st, const float* row_w, const float* norm) {
   if (H % 8 || reinterpret_cast<uintptr_t>(d_xf) % 16 || reinterpret_cast<uintptr_t>(E) % 16)
     return cudaErrorInvalidValue;
   float* row_loss = row_loss_and_sum;
   launch_pdl(ce_stream_finish_kernel, (M + kRowWarps - 1) / kRowWarps, kRowWarps * 32, 0, st, part_ref, part_sum,
-             tgt_logit, ref, valid, targets, E, M, H, V, slots, gscale, lse, row_loss, d_xf);
-  launch_pdl(sum_kernel, 1, 1024, 0, st, row_loss, M, row_loss_and_sum + M);
+             tgt_logit, ref, valid, targets, E, M, H, V, slots, gscale, row_w, norm, lse, row_loss, d_xf);
+  if (!row_w) launch_pdl(sum_kernel, 1, 1024, 0, st, row_loss, M, row_loss_and_sum + M);
+  return cudaGetLastError();
+}
+
+cudaError_t scored_rows(uint8_t* mask, const int* targets, int M, int V, cudaStream_t st) {
+  launch_pdl(scored_rows_kernel, (M + 255) / 256, 256, 0, st, mask, targets, M, V);
+  return cudaGetLastError();
+}
+
+cudaError_t loss_norm(const float* w, int M, const float* loss, int n, float* norm, float* total, cudaStream_t st) {
+  launch_pdl(loss_norm_kernel, 1, 1024, 0, st, w, M, loss, n, norm, total);
   return cudaGetLastError();
 }
 

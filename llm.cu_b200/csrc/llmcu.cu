@@ -119,6 +119,13 @@ struct llmcu_ctx {
   size_t pc_elems = 0;
   float* d_xf = nullptr;
   int ce_slots = 0;
+  // preference tuning: log-probabilities of the step, of the samples and of the
+  // reference, advantages, dL/dlogp ([max_batch * max_seq] each), per-pair
+  // losses, per-row rewards, the policy loss's stats, the gradients' power of
+  // two and its inverse, and the policy loss's workspace
+  float *tl_logp = nullptr, *tl_old = nullptr, *tl_ref = nullptr, *tl_adv = nullptr, *tl_dlogp = nullptr;
+  float *tl_loss = nullptr, *tl_reward = nullptr, *tl_stats = nullptr, *tl_norm = nullptr;
+  char* tl_ws = nullptr;
   // backward scratch
   float *dres = nullptr, *dq = nullptr, *dk = nullptr, *delta = nullptr;
   float* dq_slabs = nullptr;  // deterministic mode: per-key-tile dQ partials
@@ -363,6 +370,16 @@ void carve(llmcu_ctx* c, Carver& cv) {
   c->row_loss = cv.take<float>(M + 1);
   c->ce_ref = cv.take<float>(M);
   c->valid = cv.take<uint8_t>(M);
+  c->tl_logp = cv.take<float>(M);
+  c->tl_old = cv.take<float>(M);
+  c->tl_ref = cv.take<float>(M);
+  c->tl_adv = cv.take<float>(M);
+  c->tl_dlogp = cv.take<float>(M);
+  c->tl_loss = cv.take<float>(c->rc.max_batch);
+  c->tl_reward = cv.take<float>(c->rc.max_batch);
+  c->tl_stats = cv.take<float>(4);
+  c->tl_norm = cv.take<float>(2);
+  c->tl_ws = cv.take<char>(policy_loss_workspace(c->rc.max_batch));
   const size_t v_pad = (V + 255) / 256 * 256;
   const size_t chunk = c->rc.lm_head_chunk > 0 ? std::min<size_t>(c->rc.lm_head_chunk, v_pad) : 0;
   c->pc_elems = chunk ? M * chunk : std::min(std::max(kCeChunkElems, M * 256), M * v_pad);
@@ -532,14 +549,15 @@ struct GemmWorkspaceScope {
 };
 
 // Merged weights of the current adapters, every layer (lora_merge).
-cudaError_t merge_adapters(llmcu_ctx* ctx) {
+cudaError_t merge_adapters(llmcu_ctx* ctx, const LoraDims& d) {
   MergedOut mo;
   mo.qkv = ctx->lw[0].mqkv;
   mo.o = ctx->lw[0].mo;
   mo.gu = ctx->lw[0].mgu;
   mo.d = ctx->lw[0].md;
-  return lora_merge(ctx->lp, ctx->ld, ctx->L, ctx->mw, mo, ctx->st);
+  return lora_merge(ctx->lp, d, ctx->L, ctx->mw, mo, ctx->st);
 }
+cudaError_t merge_adapters(llmcu_ctx* ctx) { return merge_adapters(ctx, ctx->ld); }
 
 // ----------------------------------------------------------------- step
 // Embedding and every layer's forward over ctx->tok ([B, S] ids on the device),
@@ -650,7 +668,49 @@ llmcu_status forward_layers(llmcu_ctx* ctx, int B, int S) {
   return LLMCU_OK;
 }
 
-llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S) {
+// A loss over the targets' log-probabilities in place of the mean
+// cross-entropy; its inputs are in the context's tl_* buffers.
+struct TokenLoss {
+  bool preference = false;  // else the policy loss
+  PreferenceArgs pref{};
+  PolicyArgs policy{};
+};
+
+// Loss and dL/dlogp of the step's log-probabilities (tl_logp), the gradients'
+// power of two (tl_norm) and the loss's sum at row_loss[M].
+llmcu_status run_token_loss(llmcu_ctx* ctx, const TokenLoss& tl, int B, int S) {
+  cudaStream_t st = ctx->st;
+  const int M = B * S;
+  CK(ce_stream_logp(ctx->part_ref, ctx->part_sum, ctx->tgt_logit, ctx->tgt, ctx->xf, ctx->E, M, ctx->H, ctx->V,
+                    ctx->ce_slots, ctx->tl_logp, st));
+  if (tl.preference) {
+    PreferenceArgs a = tl.pref;
+    a.logp = ctx->tl_logp;
+    a.mask = ctx->valid;
+    a.loss = ctx->tl_loss;
+    a.reward = ctx->tl_reward;
+    a.dlogp = ctx->tl_dlogp;
+    a.pairs = B / 2;
+    a.seq = a.ld = S;
+    CK(preference_loss(a, st));
+    CK(loss_norm(ctx->tl_dlogp, M, ctx->tl_loss, a.pairs, ctx->tl_norm, ctx->row_loss + M, st));
+  } else {
+    PolicyArgs a = tl.policy;
+    a.logp = ctx->tl_logp;
+    a.old = ctx->tl_old;
+    a.adv = ctx->tl_adv;
+    a.mask = ctx->valid;
+    a.stats = ctx->tl_stats;
+    a.dlogp = ctx->tl_dlogp;
+    a.batch = B;
+    a.seq = a.ld = S;
+    CK(policy_loss(a, ctx->tl_ws, st));
+    CK(loss_norm(ctx->tl_dlogp, M, ctx->tl_stats, 1, ctx->tl_norm, ctx->row_loss + M, st));
+  }
+  return LLMCU_OK;
+}
+
+llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S, const TokenLoss* tl = nullptr) {
   const int M = B * S;
   const int H = ctx->H, Q = ctx->Q, KV = ctx->KV, QKV = ctx->QKV, I = ctx->I, V = ctx->V;
   const float eps = ctx->m.rms_eps;
@@ -661,7 +721,9 @@ llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S) {
   const int n_valid_local = ctx->rc.loss_all_positions ? M : B * (S - 1);
   const double n_valid_total = static_cast<double>(n_valid_local) * ctx->world;
   ctx->last_n_valid = n_valid_local;
-  const float unscale = static_cast<float>(1.0 / (kGradScale * n_valid_total));
+  // a token loss's gradient is complete but for the mean over ranks (and the
+  // power of two that tl_norm[1] takes out again)
+  const float unscale = static_cast<float>(1.0 / (kGradScale * (tl ? ctx->world : n_valid_total)));
 
   // the gradients start at zero (lora_grad stores every adapter it trains);
   // this first kernel follows the host's token upload, so it is launched
@@ -677,7 +739,10 @@ llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S) {
   set_pdl(true);
   // merged q/k/v/o weights of this step's adapters, every layer
   TIMEDN(P_LORA_PREP, d.has_mlp() ? 6 : 3, merge_adapters(ctx));
-  TIMED(P_FILL, ce_valid_rows(ctx->valid, ctx->tgt, B, S, ctx->rc.loss_all_positions, V, err, st));
+  if (tl)
+    TIMED(P_FILL, scored_rows(ctx->valid, ctx->tgt, M, V, st));
+  else
+    TIMED(P_FILL, ce_valid_rows(ctx->valid, ctx->tgt, B, S, ctx->rc.loss_all_positions, V, err, st));
   CKS(forward_layers(ctx, B, S));
   const __half* E = ctx->E;
 
@@ -707,7 +772,7 @@ llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S) {
         ctx->rc.deterministic
             ? 1
             : std::max(kLmSplitK, std::min(16, gemm_num_sms() / std::max(1, (M + 127) / 128 * ((H + 255) / 256))));
-    int launches = 2;  // + ce_stream_finish's two
+    int launches = tl ? 5 : 2;  // + ce_stream_finish's two, or its one and about four of the loss
     for (int v0 = 0; v0 < V; v0 += (v0 == 0 ? vc0 : vc)) launches += 3;
     // one event pair around the whole section (per-kernel events would break
     // the programmatic-launch overlap of its short kernels)
@@ -737,8 +802,10 @@ llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S) {
       CK(gemm(op(ctx->pc, M, n, vc), op_mn(Ec, n, H, H), M, H, Epi::kStoreF32, eb, err, st));
       v0 += n;
     }
+    if (tl) CKS(run_token_loss(ctx, *tl, B, S));
     CK(ce_stream_finish(ctx->part_ref, ctx->part_sum, ctx->tgt_logit, ctx->ce_ref, ctx->valid, ctx->tgt, E, M, H, V,
-                        ctx->ce_slots, kGradScale, ctx->lse_ce, ctx->row_loss, ctx->d_xf, st));
+                        ctx->ce_slots, kGradScale, ctx->lse_ce, ctx->row_loss, ctx->d_xf, st,
+                        tl ? ctx->tl_dlogp : nullptr, tl ? ctx->tl_norm : nullptr));
     prof_mark(ctx, P_LMHEAD, launches);
   }
   // an INT8 base's down-projection row scales ride in the fp16 gradient that
@@ -767,6 +834,7 @@ llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S) {
     gb.ws = ctx->lg_ws;
     gb.ws_floats = kLgWsFloats;
     gb.err = err;
+    gb.dev_scale = tl ? ctx->tl_norm + 1 : nullptr;
     set_pdl(!split);
     TIMEDN(P_LORA_GRAD, lora_grad_splits(M, gb) > 1 ? 2 : 1, lora_grad(gb, M, gs));
     set_pdl(true);
@@ -970,7 +1038,8 @@ llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S) {
   }
   prof_mark(ctx, P_DP_WAIT, 0);
   prof_mark(ctx, P_FILL);
-  scale_loss_kernel<<<1, 1, 0, st>>>(total, static_cast<float>(1.0 / n_valid_total), ctx->loss_dev);
+  const double loss_n = !tl ? n_valid_total : static_cast<double>(ctx->world) * (tl->preference ? B / 2 : 1);
+  scale_loss_kernel<<<1, 1, 0, st>>>(total, static_cast<float>(1.0 / loss_n), ctx->loss_dev);
   CK(cudaGetLastError());
   prof_mark(ctx, P_FILL);
   return LLMCU_OK;
@@ -997,6 +1066,59 @@ llmcu_status upload_tokens(llmcu_ctx* ctx, const int32_t* tokens, const int32_t*
   CK(cudaMemcpyAsync(ctx->tok, tokens, sizeof(int) * M, cudaMemcpyHostToDevice, ctx->st));
   CK(cudaMemcpyAsync(ctx->tgt, targets, sizeof(int) * M, cudaMemcpyHostToDevice, ctx->st));
   return LLMCU_OK;
+}
+
+// --------------------------------------- checks of the preference-tuning configs
+bool preference_args(const llmcu_preference_cfg* cfg, PreferenceArgs* a) {
+  if (!cfg || cfg->kind < LLMCU_PREF_SIGMOID || cfg->kind > LLMCU_PREF_SQUARED || !(cfg->beta > 0.f) ||
+      !std::isfinite(cfg->beta) || !(cfg->label_smoothing >= 0.f && cfg->label_smoothing <= 0.5f) ||
+      (cfg->label_smoothing != 0.f && cfg->kind != LLMCU_PREF_SIGMOID) || !std::isfinite(cfg->margin) ||
+      (cfg->margin != 0.f && cfg->kind == LLMCU_PREF_SQUARED) || (cfg->mean_tokens != 0 && cfg->mean_tokens != 1))
+    return false;
+  a->kind = cfg->kind;
+  a->beta = cfg->beta;
+  a->smoothing = cfg->label_smoothing;
+  a->margin = cfg->margin;
+  a->mean_tokens = cfg->mean_tokens;
+  return true;
+}
+
+bool policy_args(const llmcu_policy_cfg* cfg, PolicyArgs* a) {
+  if (!cfg || !(cfg->clip_low >= 0.f) || !(cfg->clip_high >= 0.f) || !std::isfinite(cfg->clip_low) ||
+      !std::isfinite(cfg->clip_high) || !(cfg->kl_beta >= 0.f) || !std::isfinite(cfg->kl_beta) ||
+      !(cfg->dual_clip == 0.f || cfg->dual_clip > 1.f) || !std::isfinite(cfg->dual_clip) ||
+      cfg->agg < LLMCU_POLICY_TOKEN_MEAN || cfg->agg > LLMCU_POLICY_CONSTANT ||
+      (cfg->agg == LLMCU_POLICY_CONSTANT && (!(cfg->norm > 0.f) || !std::isfinite(cfg->norm))) ||
+      (cfg->token_advantages != 0 && cfg->token_advantages != 1))
+    return false;
+  a->agg = cfg->agg;
+  a->token_adv = cfg->token_advantages;
+  a->beta = cfg->kl_beta;
+  a->inv_norm = cfg->agg == LLMCU_POLICY_CONSTANT ? static_cast<float>(1.0 / cfg->norm) : 0.f;
+  const double low = 1.0 - cfg->clip_low, high = 1.0 + cfg->clip_high;
+  a->low = static_cast<float>(low);
+  a->high = static_cast<float>(high);
+  a->dual = cfg->dual_clip;
+  // a ratio is never below 1 - clip_low where that is 0 or less
+  a->log_low = low > 0.0 ? std::log1p(-static_cast<double>(cfg->clip_low)) : -INFINITY;
+  a->log_high = std::log1p(static_cast<double>(cfg->clip_high));
+  a->log_dual = cfg->dual_clip > 0.f ? std::log(static_cast<double>(cfg->dual_clip)) : INFINITY;
+  return true;
+}
+
+bool muon_args(const llmcu_muon_cfg* cfg, MuonArgs* a) {
+  if (!cfg || !std::isfinite(cfg->lr) || !std::isfinite(cfg->momentum) || !std::isfinite(cfg->weight_decay) ||
+      !(cfg->eps > 0.f) || !std::isfinite(cfg->eps) || cfg->ns_steps < 1 || cfg->ns_steps > 16 ||
+      (cfg->nesterov != 0 && cfg->nesterov != 1) || (cfg->match_rms != 0 && cfg->match_rms != 1))
+    return false;
+  a->lr = cfg->lr;
+  a->momentum = cfg->momentum;
+  a->weight_decay = cfg->weight_decay;
+  a->eps = cfg->eps;
+  a->nesterov = cfg->nesterov;
+  a->match_rms = cfg->match_rms;
+  a->steps = cfg->ns_steps;
+  return true;
 }
 
 llmcu_status read_loss(llmcu_ctx* ctx, float* loss_out) {
@@ -1443,6 +1565,106 @@ llmcu_status llmcu_train_step_device(llmcu_ctx* ctx, const int32_t* d_tokens, co
   CK(cudaMemcpyAsync(ctx->tgt, d_targets, sizeof(int) * M, cudaMemcpyDeviceToDevice, ctx->st));
   CKS(run_forward_backward(ctx, batch, seq));
   CKS(do_adamw(ctx, opt, step));
+  return LLMCU_OK;
+}
+
+// ------------------------------------------------------ preference tuning
+
+llmcu_status llmcu_score(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* targets, int batch, int seq,
+                         int adapters, float* logp) {
+  if (!ctx) return LLMCU_ERR_INVALID_ARG;
+  if (!logp || (adapters != 0 && adapters != 1))
+    return fail(ctx, LLMCU_ERR_INVALID_ARG, "score: null output, or adapters not 0 or 1");
+  CK(cudaSetDevice(ctx->device));
+  CKS(validate_step(ctx, batch, seq));
+  const int M = batch * seq, H = ctx->H;
+  CKS(upload_tokens(ctx, tokens, targets, M));
+  struct PdlScope {
+    ~PdlScope() { set_pdl(false); }
+  } pdl_scope;
+  set_pdl(false);
+  GemmWorkspaceScope gws(ctx);
+  CK(cudaMemsetAsync(ctx->fx_cnt, 0, sizeof(int) * kFxCounters, ctx->st));
+  LoraDims d = ctx->ld;
+  if (!adapters) d.scale = 0.f;  // merged weights W + 0 B A: the base model
+  CK(merge_adapters(ctx, d));
+  set_pdl(true);
+  CKS(forward_layers(ctx, batch, seq));
+  TIMED(P_NORM, rmsnorm_forward(ctx->resid[ctx->L], ctx->final_norm, ctx->xf, M, H, ctx->m.rms_eps, ctx->st));
+  // the streamed head's partials hold the (max, sum) pairs: part_ref and part_sum lie together
+  TIMEDN(P_LMHEAD, 2, lm_logprobs(ctx->xf, ctx->E, ctx->tgt, ctx->tl_logp, ctx->lse_ce, M, H, ctx->V, H, H,
+                                  reinterpret_cast<float2*>(ctx->part_ref), ctx->tgt_logit, ctx->derr, ctx->st));
+  set_pdl(false);
+  CK(cudaMemcpyAsync(logp, ctx->tl_logp, sizeof(float) * M, cudaMemcpyDeviceToHost, ctx->st));
+  CK(cudaEventRecord(ctx->ev_step_done, ctx->st));
+  CKS(wait_event(ctx, ctx->ev_step_done));
+  return check_dev_err(ctx);
+}
+
+llmcu_status llmcu_preference_forward_backward(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* targets,
+                                               const float* ref_logp, int batch, int seq,
+                                               const llmcu_preference_cfg* cfg, float* loss_out, float* rewards) {
+  if (!ctx) return LLMCU_ERR_INVALID_ARG;
+  TokenLoss tl;
+  tl.preference = true;
+  if (!preference_args(cfg, &tl.pref)) return fail(ctx, LLMCU_ERR_INVALID_ARG, "preference: invalid config");
+  if (batch % 2) return fail(ctx, LLMCU_ERR_INVALID_ARG, "preference: batch %d is not a number of pairs", batch);
+  CK(cudaSetDevice(ctx->device));
+  CKS(validate_step(ctx, batch, seq));
+  const int M = batch * seq;
+  CKS(upload_tokens(ctx, tokens, targets, M));
+  if (ref_logp) {
+    CK(cudaMemcpyAsync(ctx->tl_ref, ref_logp, sizeof(float) * M, cudaMemcpyHostToDevice, ctx->st));
+    tl.pref.ref = ctx->tl_ref;
+  }
+  CKS(run_forward_backward(ctx, batch, seq, &tl));
+  if (rewards)
+    CK(cudaMemcpyAsync(rewards, ctx->tl_reward, sizeof(float) * batch, cudaMemcpyDeviceToHost, ctx->st));
+  return read_loss(ctx, loss_out);
+}
+
+llmcu_status llmcu_policy_forward_backward(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* targets,
+                                           const float* old_logp, const float* ref_logp, const float* advantages,
+                                           int batch, int seq, const llmcu_policy_cfg* cfg, float* loss_out,
+                                           float* stats) {
+  if (!ctx) return LLMCU_ERR_INVALID_ARG;
+  TokenLoss tl;
+  if (!policy_args(cfg, &tl.policy)) return fail(ctx, LLMCU_ERR_INVALID_ARG, "policy: invalid config");
+  if (!old_logp || !advantages) return fail(ctx, LLMCU_ERR_INVALID_ARG, "policy: null old_logp or advantages");
+  CK(cudaSetDevice(ctx->device));
+  CKS(validate_step(ctx, batch, seq));
+  const int M = batch * seq;
+  CKS(upload_tokens(ctx, tokens, targets, M));
+  CK(cudaMemcpyAsync(ctx->tl_old, old_logp, sizeof(float) * M, cudaMemcpyHostToDevice, ctx->st));
+  CK(cudaMemcpyAsync(ctx->tl_adv, advantages, sizeof(float) * (cfg->token_advantages ? M : batch),
+                     cudaMemcpyHostToDevice, ctx->st));
+  if (ref_logp) {
+    CK(cudaMemcpyAsync(ctx->tl_ref, ref_logp, sizeof(float) * M, cudaMemcpyHostToDevice, ctx->st));
+    tl.policy.ref = ctx->tl_ref;
+  }
+  CKS(run_forward_backward(ctx, batch, seq, &tl));
+  if (stats) CK(cudaMemcpyAsync(stats, ctx->tl_stats, 4 * sizeof(float), cudaMemcpyDeviceToHost, ctx->st));
+  return read_loss(ctx, loss_out);
+}
+
+llmcu_status llmcu_muon(llmcu_ctx* ctx, const llmcu_muon_cfg* cfg) {
+  if (!ctx) return LLMCU_ERR_INVALID_ARG;
+  MuonArgs a{};
+  if (!muon_args(cfg, &a)) return fail(ctx, LLMCU_ERR_INVALID_ARG, "muon: invalid config");
+  CK(cudaSetDevice(ctx->device));
+  const LoraDims& d = ctx->ld;
+  a.w = ctx->lp;
+  a.grad = ctx->lg;
+  a.mom = ctx->lm;
+  a.layers = ctx->L;
+  a.layer_stride = d.per_layer;
+  for (int p = 0; p < kNumProj; ++p) {
+    if (!d.has(p)) continue;
+    a.slot[a.n_slots++] = MuonSlot{d.offA(p), d.r, d.d_in(p)};
+    a.slot[a.n_slots++] = MuonSlot{d.offB(p), d.d_out(p), d.r};
+  }
+  TIMED(P_ADAMW, muon_update(a, ctx->st));
+  CK(cudaStreamSynchronize(ctx->st));
   return LLMCU_OK;
 }
 
@@ -2048,20 +2270,6 @@ llmcu_status llmcu_lm_logprobs_bwd(const void* x, const void* E, const int32_t* 
                                             workspace, d_err, static_cast<cudaStream_t>(stream)));
 }
 
-static bool preference_args(const llmcu_preference_cfg* cfg, PreferenceArgs* a) {
-  if (!cfg || cfg->kind < LLMCU_PREF_SIGMOID || cfg->kind > LLMCU_PREF_SQUARED || !(cfg->beta > 0.f) ||
-      !std::isfinite(cfg->beta) || !(cfg->label_smoothing >= 0.f && cfg->label_smoothing <= 0.5f) ||
-      (cfg->label_smoothing != 0.f && cfg->kind != LLMCU_PREF_SIGMOID) || !std::isfinite(cfg->margin) ||
-      (cfg->margin != 0.f && cfg->kind == LLMCU_PREF_SQUARED) || (cfg->mean_tokens != 0 && cfg->mean_tokens != 1))
-    return false;
-  a->kind = cfg->kind;
-  a->beta = cfg->beta;
-  a->smoothing = cfg->label_smoothing;
-  a->margin = cfg->margin;
-  a->mean_tokens = cfg->mean_tokens;
-  return true;
-}
-
 llmcu_status llmcu_preference_loss(const llmcu_preference_cfg* cfg, const float* logp, const float* ref_logp,
                                    const uint8_t* mask, const float* dloss, float* loss, float* reward, float* dlogp,
                                    int pairs, int seq, int ld, void* stream) {
@@ -2080,29 +2288,6 @@ llmcu_status llmcu_preference_loss(const llmcu_preference_cfg* cfg, const float*
   a.seq = seq;
   a.ld = ld;
   return kernel_status(preference_loss(a, static_cast<cudaStream_t>(stream)));
-}
-
-static bool policy_args(const llmcu_policy_cfg* cfg, PolicyArgs* a) {
-  if (!cfg || !(cfg->clip_low >= 0.f) || !(cfg->clip_high >= 0.f) || !std::isfinite(cfg->clip_low) ||
-      !std::isfinite(cfg->clip_high) || !(cfg->kl_beta >= 0.f) || !std::isfinite(cfg->kl_beta) ||
-      !(cfg->dual_clip == 0.f || cfg->dual_clip > 1.f) || !std::isfinite(cfg->dual_clip) ||
-      cfg->agg < LLMCU_POLICY_TOKEN_MEAN || cfg->agg > LLMCU_POLICY_CONSTANT ||
-      (cfg->agg == LLMCU_POLICY_CONSTANT && (!(cfg->norm > 0.f) || !std::isfinite(cfg->norm))) ||
-      (cfg->token_advantages != 0 && cfg->token_advantages != 1))
-    return false;
-  a->agg = cfg->agg;
-  a->token_adv = cfg->token_advantages;
-  a->beta = cfg->kl_beta;
-  a->inv_norm = cfg->agg == LLMCU_POLICY_CONSTANT ? static_cast<float>(1.0 / cfg->norm) : 0.f;
-  const double low = 1.0 - cfg->clip_low, high = 1.0 + cfg->clip_high;
-  a->low = static_cast<float>(low);
-  a->high = static_cast<float>(high);
-  a->dual = cfg->dual_clip;
-  // a ratio is never below 1 - clip_low where that is 0 or less
-  a->log_low = low > 0.0 ? std::log1p(-static_cast<double>(cfg->clip_low)) : -INFINITY;
-  a->log_high = std::log1p(static_cast<double>(cfg->clip_high));
-  a->log_dual = cfg->dual_clip > 0.f ? std::log(static_cast<double>(cfg->dual_clip)) : INFINITY;
-  return true;
 }
 
 size_t llmcu_policy_loss_workspace(int batch, int seq) {
@@ -2130,21 +2315,6 @@ llmcu_status llmcu_policy_loss(const llmcu_policy_cfg* cfg, const float* logp, c
   a.seq = seq;
   a.ld = ld;
   return kernel_status(policy_loss(a, workspace, static_cast<cudaStream_t>(stream)));
-}
-
-static bool muon_args(const llmcu_muon_cfg* cfg, MuonArgs* a) {
-  if (!cfg || !std::isfinite(cfg->lr) || !std::isfinite(cfg->momentum) || !std::isfinite(cfg->weight_decay) ||
-      !(cfg->eps > 0.f) || !std::isfinite(cfg->eps) || cfg->ns_steps < 1 || cfg->ns_steps > 16 ||
-      (cfg->nesterov != 0 && cfg->nesterov != 1) || (cfg->match_rms != 0 && cfg->match_rms != 1))
-    return false;
-  a->lr = cfg->lr;
-  a->momentum = cfg->momentum;
-  a->weight_decay = cfg->weight_decay;
-  a->eps = cfg->eps;
-  a->nesterov = cfg->nesterov;
-  a->match_rms = cfg->match_rms;
-  a->steps = cfg->ns_steps;
-  return true;
 }
 
 llmcu_status llmcu_muon_update(const llmcu_muon_cfg* cfg, float* w, const float* grad, float* momentum, int count,

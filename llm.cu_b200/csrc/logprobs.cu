@@ -100,6 +100,40 @@ __global__ void __launch_bounds__(kRows* kWarps)
   }
 }
 
+// The same for the training step's streamed head, whose partials lie [row][slot]
+// as separate references and sums: a warp a row.
+constexpr int kStreamWarps = 8;
+__global__ void __launch_bounds__(32 * kStreamWarps)
+    stream_logp_kernel(const float* __restrict__ part_ref, const float* __restrict__ part_sum,
+                       const float* __restrict__ tgt_logit, const int* __restrict__ targets,
+                       const __half* __restrict__ x, const __half* __restrict__ E, int M, int H, int V, int slots,
+                       float* __restrict__ logp) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int m = blockIdx.x * kStreamWarps + (threadIdx.x >> 5);
+  if (m >= M) return;
+  const int t = targets[m];
+  if (t < 0 || t >= V) {
+    if (lane == 0) logp[m] = 0.f;
+    return;
+  }
+  const float exact = target_logit(x + static_cast<size_t>(m) * H, E + static_cast<size_t>(t) * H, H, lane);
+  const float* pr = part_ref + static_cast<size_t>(m) * slots;
+  const float* ps = part_sum + static_cast<size_t>(m) * slots;
+  float mx = -INFINITY;
+  for (int i = lane; i < slots; i += 32) mx = fmaxf(mx, pr[i]);
+  mx = warp_max(mx);
+  float s = 0.f;
+  for (int i = lane; i < slots; i += 32) s += ps[i] * exp2f((pr[i] - mx) * kLog2e);
+  s = warp_sum(s);
+  if (lane == 0) {
+    const float rough = tgt_logit[m], d = exact - rough;
+    if (isfinite(d)) s = fmaf(exp2f((rough - mx) * kLog2e), expm1f(d), s);
+    logp[m] = exact - (mx + logf(s));
+  }
+}
+
 // dx row m from the K slices' partial sums (slab k: rows [k * slab_rows, ...)
 // of acc), in slice order, and the target's own term in fp32.
 __global__ void __launch_bounds__(256)
@@ -214,12 +248,18 @@ size_t lm_logprobs_workspace(int M, int H, int V, bool backward) {
 
 cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, float* logp, float* lse, int M, int H,
                         int V, int ldx, int lde, void* ws, int* err, cudaStream_t st) {
-  const int slots = (V + 127) / 128;
   char* w = static_cast<char*>(ws);
+  return lm_logprobs(x, E, targets, logp, lse, M, H, V, ldx, lde,
+                     reinterpret_cast<float2*>(w + up256(sizeof(float) * M)), reinterpret_cast<float*>(w), err, st);
+}
+
+cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, float* logp, float* lse, int M, int H,
+                        int V, int ldx, int lde, float2* part, float* tgt_logit, int* err, cudaStream_t st) {
+  const int slots = (V + 127) / 128;
   EpiArgs ea;
   ea.targets = targets;
-  ea.tgt_logit = reinterpret_cast<float*>(w);
-  ea.part2 = reinterpret_cast<float2*>(w + up256(sizeof(float) * M));
+  ea.tgt_logit = tgt_logit;
+  ea.part2 = part;
   PdlScope scope;
   set_pdl(false);
   cudaError_t e = gemm(Operand{x, M, H, ldx}, Operand{E, V, H, lde}, M, V, Epi::kLogProb, ea, err, st, 256);
@@ -262,6 +302,13 @@ cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* ta
   }
   return launch_pdl(logprob_dx_kernel, M, 256, 0, st, acc, p.slabs, p.slab_rows, p.ld_acc, x, ldx, E, lde, lse,
                     dlogp, targets, H, V, scale, dx, lddx);
+}
+
+cudaError_t ce_stream_logp(const float* part_ref, const float* part_sum, const float* tgt_logit, const int* targets,
+                           const __half* xf, const __half* E, int M, int H, int V, int slots, float* logp,
+                           cudaStream_t st) {
+  return launch_pdl(stream_logp_kernel, (M + kStreamWarps - 1) / kStreamWarps, 32 * kStreamWarps, 0, st, part_ref,
+                    part_sum, tgt_logit, targets, xf, E, M, H, V, slots, logp);
 }
 
 }  // namespace llmcu

@@ -434,20 +434,24 @@ constexpr int kLgUBytes = kLgM * kLgA * 2;  // 16 KB: two [64 m][64 a] TMA boxes
 constexpr int kLgWBytes = kLgM * 64 * 2;    // 8 KB: one [64 m][64 b] TMA box
 constexpr int kLgSmem = kLgStages * (kLgUBytes + kLgWBytes) + 1024 + 256;
 
+__device__ __forceinline__ float lg_scale(const LoraGradProb& pb, const LoraGradBatch& batch) {
+  return batch.dev_scale ? pb.scale * __ldg(batch.dev_scale) : pb.scale;
+}
+
 // Stores one a-tile's final sums into the problem's gradients: acc[16 g + b]
-// of a-row ar (of the tile at a0) times the problem's scale.  [a][b]
+// of a-row ar (of the tile at a0) times `scale`.  [a][b]
 // row-major gradients (dB: sa = 16, sb = 1) are staged through shared memory
 // `stage` ([128][17] floats) so that the stores leave as contiguous runs; the
 // [b][a] ones (dA: sa = 1) are already contiguous across the lanes.  The
 // staged case synchronises the CTA (its condition is CTA-uniform).
-__device__ __forceinline__ void lg_store(const LoraGradProb& pb, int a0, int sel, int ar, const float (&acc)[64],
-                                         float* stage) {
+__device__ __forceinline__ void lg_store(const LoraGradProb& pb, float scale, int a0, int sel, int ar,
+                                         const float (&acc)[64], float* stage) {
   const int ng = pb.groups;
   const int a = a0 + ar;
   const bool staged = pb.sb == 1 && pb.sa == 16 && pb.Bn == 16 && (ng == 1 || pb.ilv) && a0 + 128 <= pb.A;
   if (staged) {  // group sel's 16 columns
 #pragma unroll
-    for (int j = 0; j < 16; ++j) stage[ar * 17 + j] = (sel ? acc[16 + j] : acc[j]) * pb.scale;
+    for (int j = 0; j < 16; ++j) stage[ar * 17 + j] = (sel ? acc[16 + j] : acc[j]) * scale;
     __syncthreads();
     float* dst = pb.out[sel] + static_cast<size_t>(pb.ilv ? ((a0 >> 8) << 7) : a0) * 16;
     for (int i = threadIdx.x; i < 128 * 16; i += blockDim.x) dst[i] = stage[(i >> 4) * 17 + (i & 15)];
@@ -458,7 +462,7 @@ __device__ __forceinline__ void lg_store(const LoraGradProb& pb, int a0, int sel
     for (int bcol = 0; bcol < 64; ++bcol) {
       const int g = bcol >> 4, b = bcol & 15;
       if (g < ng && b < pb.Bn && pb.out[g] && (!pb.ilv || g == sel))
-        pb.out[g][static_cast<size_t>(orow) * pb.sa + static_cast<size_t>(b) * pb.sb] = acc[bcol] * pb.scale;
+        pb.out[g][static_cast<size_t>(orow) * pb.sa + static_cast<size_t>(b) * pb.sb] = acc[bcol] * scale;
     }
   }
 }
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(kLgThreads, 2)
       for (int j = 0; j < 64; ++j)
         if (j < ncol) mine[j * kLgA + ar] = acc[j];
     } else {
-      lg_store(pb, a0, sel, ar, acc, reinterpret_cast<float*>(smem));  // the stage buffers are idle now
+      lg_store(pb, lg_scale(pb, batch), a0, sel, ar, acc, reinterpret_cast<float*>(smem));  // the stage buffers are idle now
     }
   }
   tc_fence_before();
@@ -640,7 +644,7 @@ __global__ void __launch_bounds__(256) lora_grad_reduce_kernel(const LoraGradBat
   const int a = a0 + ar;
   if (a < pb.A && b < pb.Bn && pb.out[g] && (!pb.ilv || g == sel)) {
     const int orow = pb.ilv ? ((a0 >> 8) << 7) + ar : a;  // the interleave maps a to its adapter row
-    pb.out[g][static_cast<size_t>(orow) * pb.sa + static_cast<size_t>(b) * pb.sb] = t * pb.scale;
+    pb.out[g][static_cast<size_t>(orow) * pb.sa + static_cast<size_t>(b) * pb.sb] = t * lg_scale(pb, batch);
   }
 }
 

@@ -112,6 +112,7 @@ struct LoraGradBatch {
   float* ws = nullptr;
   size_t ws_floats = 0;
   int* err = nullptr;
+  const float* dev_scale = nullptr;  // every problem's scale times *dev_scale (null: 1)
 };
 
 cudaError_t lora_merge(const float* flat, const LoraDims& d, int n_layers, const MergeWeights& base,

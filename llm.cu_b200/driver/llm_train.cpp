@@ -17,7 +17,10 @@
 // --rank R / --alpha A (LoRA rank 1..16 and alpha; default the config's),
 // --lora-targets LIST (comma-separated wq,wk,wv,wo,w_gate,w_up,w_down, or
 // "attn" = the reference's q/k/v/o, "mlp", "all"; default attn),
-// --int8-in-gemm (with --int8: the GEMMs stage the INT8 codes themselves).
+// --int8-in-gemm (with --int8: the GEMMs stage the INT8 codes themselves),
+// --optimizer adamw|muon (default adamw; muon orthogonalises each adapter's
+// momentum, Nesterov, at 0.2 sqrt(max(rows, cols)), so that AdamW's learning
+// rates carry over; its momentum travels in the same sidecar).
 // Data parallel: when WORLD_SIZE > 1 (e.g. under torchrun) each process
 // drives GPU LOCAL_RANK, rank 0 writes the NCCL id to --dp-id-file and the
 // others read it; rank r takes sequences r, r+W, ... of every step window.
@@ -60,7 +63,7 @@ int main(int argc, char** argv) {
   unsigned long long seed = 1234;
   int lora_rank = 0;
   float lora_alpha = 0.f;
-  std::string targets_arg = "attn";
+  std::string targets_arg = "attn", optimizer = "adamw";
 
   for (int i = 1; i < argc; i++) {
     auto next = [&](const char* flag) -> const char* {
@@ -84,6 +87,7 @@ int main(int argc, char** argv) {
     else if ((v = next("--rank"))) lora_rank = atoi(v);
     else if ((v = next("--alpha"))) lora_alpha = static_cast<float>(atof(v));
     else if ((v = next("--lora-targets"))) targets_arg = v;
+    else if ((v = next("--optimizer"))) optimizer = v;
     else if (!strcmp(argv[i], "--synthetic")) synthetic = true;
     else if (!strcmp(argv[i], "--int8")) int8 = true;
     else if (!strcmp(argv[i], "--int8-in-gemm")) int8_in_gemm = true;
@@ -92,10 +96,15 @@ int main(int argc, char** argv) {
              "                 [--batch B] [--config tiny|1.7b] [--synthetic] [--int8] [--weights DIR]\n"
              "                 [--data FILE] [--out DIR] [--seed N] [--dp-id-file PATH] [--resume N]\n"
              "                 [--rank R] [--alpha A] [--lora-targets attn|mlp|all|wq,wk,...,w_down]\n"
-             "                 [--int8-in-gemm]\n");
+             "                 [--int8-in-gemm] [--optimizer adamw|muon]\n");
       return 0;
     }
   }
+  if (optimizer != "adamw" && optimizer != "muon") {
+    fprintf(stderr, "ERROR: unknown --optimizer '%s'\n", optimizer.c_str());
+    return 1;
+  }
+  const bool muon = optimizer == "muon";
   if (log_every < 1) log_every = 1;
   if (save_every < 1) save_every = steps;
 
@@ -222,6 +231,7 @@ int main(int argc, char** argv) {
   // the synthetic stream draws seq_len + 1 ids per sequence: skip the steps already taken
   if (synthetic && resume > 0) rng.discard(static_cast<unsigned long long>(resume) * batch * (seq_len + 1));
   const llmcu_adamw_cfg opt = {lr, beta1, beta2, eps_adam, wd};
+  const llmcu_muon_cfg muon_opt = {lr, 0.95f, wd, 1e-7f, 1, 1, 5};
   if (rank == 0) printf("\n=== Training ===\n");
   float running = 0.f;
   int count = 0;
@@ -244,8 +254,13 @@ int main(int argc, char** argv) {
       }
     }
     float loss = 0.f;
-    if ((s = llmcu_train_step(ctx, tok.data(), tgt.data(), batch, seq_len, &opt, step, &loss)) != LLMCU_OK)
+    if (muon) {
+      if ((s = llmcu_forward_backward(ctx, tok.data(), tgt.data(), batch, seq_len, &loss)) != LLMCU_OK)
+        die(ctx, s, "llmcu_forward_backward");
+      if ((s = llmcu_muon(ctx, &muon_opt)) != LLMCU_OK) die(ctx, s, "llmcu_muon");
+    } else if ((s = llmcu_train_step(ctx, tok.data(), tgt.data(), batch, seq_len, &opt, step, &loss)) != LLMCU_OK) {
       die(ctx, s, "llmcu_train_step");
+    }
     running += loss;
     ++count;
     if (step % log_every == 0 && rank == 0) {

@@ -250,6 +250,12 @@ _SIGS = {
     "llmcu_policy_loss": (C.c_int, [C.POINTER(_PolicyCfg)] + [C.c_void_p] * 7 + [C.c_int] * 3 +
                           [C.c_void_p, C.c_size_t, C.c_void_p]),
     "llmcu_muon_update": (C.c_int, [C.POINTER(_MuonCfg)] + [C.c_void_p] * 3 + [C.c_int] * 3 + [C.c_void_p]),
+    "llmcu_score": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "llmcu_preference_forward_backward": (C.c_int, [C.c_void_p] * 4 + [C.c_int, C.c_int, C.POINTER(_PreferenceCfg),
+                                                                       C.POINTER(C.c_float), C.c_void_p]),
+    "llmcu_policy_forward_backward": (C.c_int, [C.c_void_p] * 6 + [C.c_int, C.c_int, C.POINTER(_PolicyCfg),
+                                                                   C.POINTER(C.c_float), C.c_void_p]),
+    "llmcu_muon": (C.c_int, [C.c_void_p, C.POINTER(_MuonCfg)]),
     "llmcu_kernel_checks": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
     "llmcu_kernel_wait_selftest": (C.c_int, [C.c_void_p]),
     "llmcu_lora_layout_count": (C.c_int64, [C.POINTER(_LoraLayout)]),
@@ -461,6 +467,48 @@ class Context:
         loss = C.c_float()
         self._check(lib().llmcu_read_loss(self._h, C.byref(loss)), "read_loss")
         return float(loss.value)
+
+    # -- preference tuning (targets outside [0, vocab) are not scored)
+    def score(self, tokens, targets, adapters: bool = True) -> np.ndarray:
+        """Log-probabilities [B, S] of the targets (0 where not scored) under the
+        current adapters, or the base alone."""
+        t, g = self._batch(tokens, targets)
+        out = np.empty(t.shape, np.float32)
+        self._check(lib().llmcu_score(self._h, _ptr(t), _ptr(g), *t.shape, int(adapters), _ptr(out)), "score")
+        return out
+
+    @staticmethod
+    def _like(a, shape, what):
+        if a is None:
+            return None, None
+        a = np.ascontiguousarray(a, dtype=np.float32)
+        if a.shape != shape:
+            raise ValueError(f"{what} {a.shape} must be {shape}")
+        return a, _ptr(a)
+
+    def preference_forward_backward(self, tokens, targets, cfg: Preference, ref_logp=None):
+        """(mean loss, rewards [B]) of B / 2 pairs, the chosen sequences first; adapter gradients left in place."""
+        t, g = self._batch(tokens, targets)
+        ref, p_ref = self._like(ref_logp, t.shape, "ref_logp")
+        loss, rewards = C.c_float(), np.empty(t.shape[0], np.float32)
+        self._check(lib().llmcu_preference_forward_backward(self._h, _ptr(t), _ptr(g), p_ref, *t.shape, cfg.c,
+                                                            C.byref(loss), _ptr(rewards)),
+                    "preference_forward_backward")
+        return float(loss.value), rewards
+
+    def policy_forward_backward(self, tokens, targets, old_logp, advantages, cfg: Policy, ref_logp=None):
+        """(loss, {"kl", "clipped", "tokens"}); adapter gradients left in place."""
+        t, g = self._batch(tokens, targets)
+        old, p_old = self._like(old_logp, t.shape, "old_logp")
+        ref, p_ref = self._like(ref_logp, t.shape, "ref_logp")
+        adv, p_adv = self._like(advantages, t.shape if cfg.token_advantages else t.shape[:1], "advantages")
+        loss, stats = C.c_float(), np.empty(4, np.float32)
+        self._check(lib().llmcu_policy_forward_backward(self._h, _ptr(t), _ptr(g), p_old, p_ref, p_adv, *t.shape, cfg.c,
+                                                        C.byref(loss), _ptr(stats)), "policy_forward_backward")
+        return float(loss.value), {"kl": float(stats[1]), "clipped": float(stats[2]), "tokens": int(stats[3])}
+
+    def muon(self, cfg: Muon):
+        self._check(lib().llmcu_muon(self._h, cfg.c), "muon")
 
     # -- files
     def save_lora(self, directory: str, step: int):

@@ -469,6 +469,35 @@ def test_policy_small_kl_keeps_its_digits(llmcu, cuda_device):
         assert abs(g.item() + math.expm1(x)) <= (8 + 2 * abs(x)) * U * abs(math.expm1(x))
 
 
+def test_loss_gradients_by_differences(llmcu, cuda_device):
+    """Central differences of both losses along a random direction v, taken over
+    the step really made in fp32.  Second derivatives along v are under 1 (beta^2
+    |v|^2 / 4 and (|A| r + beta e^d) |v|^2), third ones too, so a step of h is
+    off by at most h^3 / 3; each loss is off by 16 roundings of 1."""
+    dev, B, S = cuda_device, 8, 24
+    lp, old, rf, adv, mask = policy_inputs(dev, B, S, S, 3, True)
+    v = torch.randn(B, S, device=dev, generator=torch.Generator(device=dev).manual_seed(1)) * mask
+    v /= v.norm() * 4
+    h = 2.0 ** -4
+    up, down = (torch.where(mask, lp + s * h * v, lp) for s in (1, -1))
+    step = torch.where(mask, up.double() - down.double(), 0.0)
+
+    def pref(x, dloss=None):
+        return run_pref(llmcu, llmcu.Preference(llmcu.PREF_SIGMOID, 0.3, 0.1), x, rf, mask, None, B // 2, S, S, dev)
+
+    # wide clips: no token changes sides within the step
+    cfg = llmcu.Policy(0.999, 50.0, 0.1, 0.0, llmcu.POLICY_TOKEN_MEAN, 1.0, True)
+
+    def policy(x):
+        return run_policy(llmcu, cfg, x, old, rf, adv, mask, B, S, S, dev)
+
+    tol = h ** 3 / 3 + 2 * 16 * U
+    diff = pref(up)[0].double().mean() - pref(down)[0].double().mean()
+    assert abs(diff - (pref(lp)[2].double() * step).sum()) <= tol
+    diff = policy(up)[0][0].double() - policy(down)[0][0].double()
+    assert abs(diff - (policy(lp)[1].double() * step).sum()) <= tol
+
+
 # ------------------------------------------------------------------ Muon update
 NS = tuple(float(v) for v in torch.tensor([3.4445, -4.7750, 2.0315]))
 
