@@ -429,7 +429,7 @@ llmcu_status llmcu_lm_logprobs(const void* x, const void* E, const int32_t* targ
 /* Its gradient for the hidden states (the head is frozen): dx[m] = scale *
  * dlogp[m] * (E[t] - sum_v exp(x[m] . E[v] - lse[m]) E[v]) as fp16 [rows,
  * hidden] with row stride lddx; 0 where the target scores nothing, whatever
- * dlogp holds there.  lse is the forward's.  `scale` (a loss scale, a power of
+ * dlogp holds there, and where dlogp is 0 (such rows cost next to nothing).  lse is the forward's.  `scale` (a loss scale, a power of
  * two as a rule) keeps small gradients in fp16's range.  Workspace:
  * llmcu_lm_logprobs_workspace(rows, hidden, vocab, 1) bytes. */
 llmcu_status llmcu_lm_logprobs_bwd(const void* x, const void* E, const int32_t* targets, const float* lse,

@@ -149,6 +149,7 @@ struct EpiArgs {
   // multiple of 256; out then has ksplit * slab_rows rows and each element one
   // writer, so the sums' order is fixed; no accumulate needed); 0: the same rows
   int slab_rows = 0;
+  const int* m_rows = nullptr;  // rows really there, on the device (null: M)
   // kStoreF16Delta: O [M, n_main] (row stride ld_o) and the delta output [B, n_heads, seq]
   const __half* attn_o = nullptr;
   int ld_o = 0;

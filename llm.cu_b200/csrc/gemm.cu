@@ -363,13 +363,14 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
   sh.fx_ws = nullptr;
   sh.fx_cnt = nullptr;
   sh.b_scale = B.mn ? nullptr : B.q8_scale;
+  sh.m_rows = ea.m_rows;
   if (ea.ksplit > 1) {  // K slices reduce-add into the same rows
     const int nk = sh.kb_per_split;
     const int kbps = (nk + ea.ksplit - 1) / ea.ksplit;
     sh.kb_per_split = kbps;
     sh.splits = (nk + kbps - 1) / kbps;
     sh.split_row_tiles = ea.slab_rows / (kBlockM * CG);
-  } else if (t_fx_ws && epi != Epi::kCEStream && epi != Epi::kLogProb && epi != Epi::kProbs) {
+  } else if (t_fx_ws && !ea.m_rows && epi != Epi::kCEStream && epi != Epi::kLogProb && epi != Epi::kProbs) {
     // tiles that fill under half a wave: K splits with a fix-up, about one
     // wave of units, at least two 64-deep K blocks each
     const int slots = CG == 2 ? g_num_sms / 2 : g_num_sms;

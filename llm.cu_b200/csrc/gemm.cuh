@@ -61,6 +61,9 @@ struct GemmShape {
   // INT8 B, K-major (Q8 forward kernels): the weight's per-row fp32 scales,
   // one per output column, applied by the epilogue
   const float* b_scale;
+  // rows really there (at most M; null: M), counted on the device by an
+  // earlier kernel: row tiles past them are not run, and M only bounds them
+  const int* m_rows;
 };
 
 constexpr int kBlockM = 128;
@@ -1063,8 +1066,9 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int nk = (sh.K + kBlockK - 1) / kBlockK;
-  const int num_units = sh.num_tiles * sh.splits;  // (tile, K split) work units
-  if (warp == 0 && lane == 0 && unit0 < num_units) {
+  int tiles_m = sh.tiles_m, num_tiles = sh.num_tiles;
+  int num_units = num_tiles * sh.splits;  // (tile, K split) work units
+  if (warp == 0 && lane == 0 && unit0 < num_units && !sh.m_rows) {
     // while the previous kernel finishes: the first unit's first stages of A
     // and B into L2.  A prefetch only fills L2, which stays coherent with that
     // kernel's writes; the loads into shared memory wait for it below.
@@ -1087,6 +1091,11 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
     }
   }
   pdl_wait();  // the prologue above overlapped the previous kernel's tail
+  if (sh.m_rows) {
+    tiles_m = min(tiles_m, (*sh.m_rows + kRowsPerTile - 1) / kRowsPerTile);
+    num_tiles = tiles_m * sh.tiles_n;
+    num_units = num_tiles * sh.splits;
+  }
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1094,10 +1103,10 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
       int it = 0;
       bool ok = true;
       for (int u = unit0; u < num_units && ok; u += ustep) {
-        const int tile = u % sh.num_tiles;
-        const int sp = u / sh.num_tiles;
-        const int tm = sh.n_fastest ? tile / sh.tiles_n : tile % sh.tiles_m;
-        const int tn = sh.n_fastest ? tile % sh.tiles_n : tile / sh.tiles_m;
+        const int tile = u % num_tiles;
+        const int sp = u / num_tiles;
+        const int tm = sh.n_fastest ? tile / sh.tiles_n : tile % tiles_m;
+        const int tn = sh.n_fastest ? tile % sh.tiles_n : tile / tiles_m;
         const int kb_end = min(nk, (sp + 1) * sh.kb_per_split);
         const int arow = tm * kRowsPerTile + static_cast<int>(rank) * kBlockM;
         const int brow = tn * BN + static_cast<int>(rank) * kBRows;
@@ -1172,7 +1181,7 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
         if (!mbar_wait(&acc_empty[acc], ((i >> 1) & 1) ^ 1, abort_flag, err, kErrWaitEpilogue)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        const int sp = u / sh.num_tiles;
+        const int sp = u / num_tiles;
         const int kb_begin = sp * sh.kb_per_split;
         const int kb_end = min(nk, kb_begin + sh.kb_per_split);
         for (int kb = kb_begin; kb < kb_end; ++kb, ++it) {
@@ -1220,7 +1229,7 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
     int it = 0;
     bool ok = true;
     for (int u = unit0; u < num_units && ok; u += ustep) {
-      const int sp = u / sh.num_tiles;
+      const int sp = u / num_tiles;
       const int kb_end = min(nk, (sp + 1) * sh.kb_per_split);
       for (int kb = sp * sh.kb_per_split; kb < kb_end; ++kb, ++it) {
         const int s = it % STAGES;
@@ -1323,10 +1332,10 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
     bool ok = true;
     for (int u = unit0; u < num_units && ok; u += ustep, ++i) {
       const int acc = i & 1;
-      const int tile = u % sh.num_tiles;
-      const int sp = u / sh.num_tiles;
-      const int tm = sh.n_fastest ? tile / sh.tiles_n : tile % sh.tiles_m;
-      const int tn = sh.n_fastest ? tile % sh.tiles_n : tile / sh.tiles_m;
+      const int tile = u % num_tiles;
+      const int sp = u / num_tiles;
+      const int tm = sh.n_fastest ? tile / sh.tiles_n : tile % tiles_m;
+      const int tn = sh.n_fastest ? tile % sh.tiles_n : tile / tiles_m;
       // split s -> its row block of partials; the odd CTA of a pair owns rows 128..255
       c.row0 = (sp * sh.split_row_tiles + tm) * kRowsPerTile + static_cast<int>(rank) * kBlockM + ew * 32;
       c.row = c.row0 + lane;

@@ -2234,6 +2234,8 @@ size_t llmcu_lm_logprobs_workspace(int rows, int hidden, int vocab, int backward
 }
 
 static bool bad_workspace(const void* ws) { return reinterpret_cast<uintptr_t>(ws) % 256 != 0; }
+// rows of fp16 that the TMA (and 16-byte loads) can read
+static bool bad_rows(const void* p, int ld) { return reinterpret_cast<uintptr_t>(p) % 16 || ld % 8; }
 static bool bad_floats(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (reinterpret_cast<uintptr_t>(p) % 4) return true;
@@ -2246,7 +2248,8 @@ llmcu_status llmcu_lm_logprobs(const void* x, const void* E, const int32_t* targ
   if (!x || !E || !targets || !logp || !lse || !workspace || rows <= 0 || hidden <= 0 || vocab <= 0 || ldx < hidden ||
       lde < hidden || workspace_bytes < lm_logprobs_workspace(rows, hidden, vocab, false))
     return LLMCU_ERR_INVALID_ARG;
-  if (bad_workspace(workspace) || bad_floats({targets, logp, lse})) return LLMCU_ERR_UNSUPPORTED;
+  if (bad_rows(x, ldx) || bad_rows(E, lde) || bad_workspace(workspace) || bad_floats({targets, logp, lse}))
+    return LLMCU_ERR_UNSUPPORTED;
   int* d_err = nullptr;
   if (kernel_err_word(&d_err) != cudaSuccess) return LLMCU_ERR_CUDA;
   return kernel_status(lm_logprobs(static_cast<const __half*>(x), static_cast<const __half*>(E), targets, logp, lse,
@@ -2261,7 +2264,8 @@ llmcu_status llmcu_lm_logprobs_bwd(const void* x, const void* E, const int32_t* 
       ldx < hidden || lde < hidden || lddx < hidden ||
       workspace_bytes < lm_logprobs_workspace(rows, hidden, vocab, true))
     return LLMCU_ERR_INVALID_ARG;
-  if (bad_workspace(workspace) || bad_floats({targets, lse, dlogp}) || reinterpret_cast<uintptr_t>(dx) % 2)
+  if (bad_rows(x, ldx) || bad_rows(E, lde) || bad_workspace(workspace) || bad_floats({targets, lse, dlogp}) ||
+      reinterpret_cast<uintptr_t>(dx) % 2)
     return LLMCU_ERR_UNSUPPORTED;
   int* d_err = nullptr;
   if (kernel_err_word(&d_err) != cudaSuccess) return LLMCU_ERR_CUDA;

@@ -18,6 +18,14 @@ namespace llmcu {
 
 namespace {
 
+// Two (max, sum of exp(l - max)) pairs as one.
+__device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
+  const float n = fmaxf(a.x, b.x);
+  // both maxima -inf: the sums are 0, or a NaN
+  const float s = n > -INFINITY ? a.y * exp2f((a.x - n) * kLog2e) + b.y * exp2f((b.x - n) * kLog2e) : a.y + b.y;
+  return make_float2(n, s);
+}
+
 // x . e in fp32 by one warp (the same order of sums wherever it is called):
 // the target's logit.  The tensor cores cut what they add to the accumulator,
 // which leaves a logit of 10 about 3e-5 short after 128 steps of K; over the
@@ -44,6 +52,152 @@ __device__ __forceinline__ float target_logit(const __half* __restrict__ x, cons
 constexpr int kRows = 32;   // rows per CTA of the forward's finishing kernel: one per lane
 constexpr int kWarps = 32;  // its warps share the slots
 
+// Few rows (M <= kFewRows): the vocabulary is read once by plain loads and
+// multiplied on the CUDA cores, in fp32.  What bounds it is reading E: 622 MB
+// for 151936 x 2048 is 95 us at the measured copy rate.  The GEMM, whose tiles
+// of 256 columns take five rounds for 4.01 rounds' worth of work there, runs
+// 133 to 138 us; this kernel 106 us for one row and 116 for two.  With four
+// rows (148 us) the products outweigh the loads.
+//
+// A warp takes four rows of E at a time, a lane eight elements of each every
+// 256; x lies in shared memory as fp32, its halves of eight apart, so that a
+// warp's 16-byte reads meet every bank once.  The four logits of each x row
+// meet in all lanes, which keep its running maximum and sum.
+constexpr int kFewRows = 2;
+constexpr int kFewThreads = 512;
+constexpr int kFewBlocks = 2;  // CTAs an SM
+constexpr int kFewSmem = 96 * 1024;
+constexpr int kVecRows = 4;    // rows of E a warp takes at once
+
+template <int MR>
+__global__ void __launch_bounds__(kFewThreads, kFewBlocks)
+    few_rows_kernel(const __half* __restrict__ x, const __half* __restrict__ E, const int* __restrict__ targets, int M,
+                    int H, int V, int ldx, int lde, float2* __restrict__ part, float* __restrict__ tgt_logit) {
+  extern __shared__ float xs[];  // [MR][h256]
+  __shared__ float2 red[kFewThreads / 32][MR];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int h256 = (H + 255) & ~255;
+  for (int e = threadIdx.x; e < MR * h256; e += kFewThreads) {
+    const int m = e / h256, k = e - m * h256;
+    const float v = m < M && k < H ? __half2float(x[static_cast<size_t>(m) * ldx + k]) : 0.f;
+    xs[m * h256 + (k & ~255) + (k & 4) * 32 + ((k & 255) >> 3) * 4 + (k & 3)] = v;
+  }
+  pdl_trigger();
+  __syncthreads();
+  float mx[MR], sum[MR];
+  int t[MR];
+#pragma unroll
+  for (int m = 0; m < MR; ++m) {
+    mx[m] = -INFINITY;
+    sum[m] = 0.f;
+    t[m] = m < M ? targets[m] : -1;
+  }
+  // a run of E's rows for each warp of the grid
+  const int warps = gridDim.x * (kFewThreads / 32);
+  const int me = blockIdx.x * (kFewThreads / 32) + w;
+  const int v_end = static_cast<int>(static_cast<int64_t>(V) * (me + 1) / warps);
+  for (int v0 = static_cast<int>(static_cast<int64_t>(V) * me / warps); v0 < v_end; v0 += kVecRows) {
+    float acc[kVecRows][MR];
+#pragma unroll
+    for (int r = 0; r < kVecRows; ++r)
+#pragma unroll
+      for (int m = 0; m < MR; ++m) acc[r][m] = 0.f;
+    const __half* row[kVecRows];  // past the run: its last row again, not used
+#pragma unroll
+    for (int r = 0; r < kVecRows; ++r) row[r] = E + static_cast<size_t>(min(v0 + r, v_end - 1)) * lde;
+#pragma unroll 2
+    for (int k0 = 0; k0 < h256; k0 += 256) {
+      const int k = k0 + lane * 8;
+      uint4 e[kVecRows];
+#pragma unroll
+      for (int r = 0; r < kVecRows; ++r) {
+        e[r] = make_uint4(0u, 0u, 0u, 0u);
+        if (k + 8 <= H) {
+          e[r] = __ldcs(reinterpret_cast<const uint4*>(row[r] + k));
+        } else if (k < H) {
+          __half* h = reinterpret_cast<__half*>(&e[r]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (k + j < H) h[j] = row[r][k + j];
+        }
+      }
+      float f[kVecRows][8];
+#pragma unroll
+      for (int r = 0; r < kVecRows; ++r) {
+        const __half2* h = reinterpret_cast<const __half2*>(&e[r]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 v = __half22float2(h[j]);
+          f[r][2 * j] = v.x;
+          f[r][2 * j + 1] = v.y;
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        const float4 a = *reinterpret_cast<const float4*>(xs + m * h256 + k0 + lane * 4);
+        const float4 b = *reinterpret_cast<const float4*>(xs + m * h256 + k0 + 128 + lane * 4);
+#pragma unroll
+        for (int r = 0; r < kVecRows; ++r) {
+          float c = acc[r][m];
+          c = fmaf(a.x, f[r][0], c);
+          c = fmaf(a.y, f[r][1], c);
+          c = fmaf(a.z, f[r][2], c);
+          c = fmaf(a.w, f[r][3], c);
+          c = fmaf(b.x, f[r][4], c);
+          c = fmaf(b.y, f[r][5], c);
+          c = fmaf(b.z, f[r][6], c);
+          acc[r][m] = fmaf(b.w, f[r][7], c);
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      float l[kVecRows];
+      float n = mx[m];
+#pragma unroll
+      for (int r = 0; r < kVecRows; ++r) {
+        const float v = warp_sum(acc[r][m]);
+        l[r] = v0 + r < v_end ? v : -INFINITY;
+        if (v0 + r == t[m] && v0 + r < v_end && lane == 0) tgt_logit[m] = v;
+        n = fmaxf(n, l[r]);
+      }
+      if (n > -INFINITY) {
+        float s = sum[m] * exp2f((mx[m] - n) * kLog2e);
+#pragma unroll
+        for (int r = 0; r < kVecRows; ++r) s += exp2f((l[r] - n) * kLog2e);
+        sum[m] = s;
+        mx[m] = n;
+      } else {  // -inf so far, or NaN: the sum keeps the NaN
+#pragma unroll
+        for (int r = 0; r < kVecRows; ++r) sum[m] += l[r] == -INFINITY ? 0.f : l[r];
+      }
+    }
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int m = 0; m < MR; ++m) red[w][m] = make_float2(mx[m], sum[m]);
+  }
+  __syncthreads();
+  if (threadIdx.x < MR && threadIdx.x < M) {
+    float2 a = red[0][threadIdx.x];
+    for (int i = 1; i < kFewThreads / 32; ++i) a = join_pairs(a, red[i][threadIdx.x]);
+    part[static_cast<size_t>(blockIdx.x) * M + threadIdx.x] = a;
+  }
+}
+
+template <int MR>
+cudaError_t few_rows(const __half* x, const __half* E, const int* targets, int M, int H, int V, int ldx, int lde,
+                     float2* part, float* tgt_logit, int blocks, cudaStream_t st) {
+  static std::atomic<unsigned long long> attr_set{0};
+  cudaError_t e = once_per_device(attr_set, [] {
+    return cudaFuncSetAttribute(few_rows_kernel<MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+  });
+  if (e != cudaSuccess) return e;
+  const size_t smem = sizeof(float) * MR * ((H + 255) & ~255);
+  return launch_pdl(few_rows_kernel<MR>, blocks, kFewThreads, smem, st, x, E, targets, M, H, V, ldx, lde, part,
+                    tgt_logit);
+}
+
 // Joins the slots' (max, sum) pairs of 32 rows: warp w takes slots w, w + 32,
 // ...; lanes are rows, so every load is 256 contiguous bytes.  Before that,
 // while the GEMM still runs, warp w forms row w's target logit (x, E and the
@@ -68,26 +222,18 @@ __global__ void __launch_bounds__(kRows* kWarps)
   }
   pdl_wait();
   const int m = blockIdx.x * kRows + lane;
-  float mx = -INFINITY, s = 0.f;
-  auto join = [&](float2 o) {
-    const float n = fmaxf(mx, o.x);
-    if (n > -INFINITY) {
-      s = s * exp2f((mx - n) * kLog2e) + o.y * exp2f((o.x - n) * kLog2e);
-    } else {
-      s += o.y;  // 0, or a NaN
-    }
-    mx = n;
-  };
+  float2 p = make_float2(-INFINITY, 0.f);
   if (m < M) {
-#pragma unroll 8
-    for (int i = w; i < slots; i += kWarps) join(__ldg(part + static_cast<size_t>(i) * M + m));
+#pragma unroll 4
+    for (int i = w; i < slots; i += kWarps) p = join_pairs(p, part[static_cast<size_t>(i) * M + m]);
   }
-  red[w][lane] = make_float2(mx, s);
+  red[w][lane] = p;
   __syncthreads();
   if (w == 0 && m < M) {
-    mx = -INFINITY;
-    s = 0.f;
-    for (int i = 0; i < kWarps; ++i) join(red[i][lane]);
+    p = red[0][lane];
+    for (int i = 1; i < kWarps; ++i) p = join_pairs(p, red[i][lane]);
+    const float mx = p.x;
+    float s = p.y;
     const int t = targets[m];
     const bool ok = t >= 0 && t < V;
     if (ok) {
@@ -134,10 +280,66 @@ __global__ void __launch_bounds__(32 * kStreamWarps)
   }
 }
 
+// The rows that have a gradient -- their target lies in the vocabulary and
+// their upstream gradient is not 0 -- in order: list[0 .. *count), and each
+// row's place there (or -1).  One CTA.
+__global__ void __launch_bounds__(1024)
+    live_rows_kernel(const int* __restrict__ targets, const float* __restrict__ dlogp, int M, int V,
+                     int* __restrict__ list, int* __restrict__ place, int* __restrict__ count) {
+  pdl_trigger();
+  __shared__ int warps[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int base = 0;
+  for (int m0 = 0; m0 < M; m0 += 1024) {
+    const int m = m0 + threadIdx.x;
+    const bool live = m < M && targets[m] >= 0 && targets[m] < V && dlogp[m] != 0.f;
+    const uint32_t b = __ballot_sync(0xffffffffu, live);
+    if (lane == 0) warps[w] = __popc(b);
+    __syncthreads();
+    int before = 0, total = 0;
+    for (int i = 0; i < 32; ++i) {
+      before += i < w ? warps[i] : 0;
+      total += warps[i];
+    }
+    const int at = base + before + __popc(b & ((1u << lane) - 1u));
+    if (live) list[at] = m;
+    if (m < M) place[m] = live ? at : -1;
+    base += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+
+// x, lse and targets of those rows, one after another (a warp a row).
+__global__ void __launch_bounds__(256)
+    gather_rows_kernel(const __half* __restrict__ x, int ldx, const float* __restrict__ lse,
+                       const int* __restrict__ targets, const int* __restrict__ list, const int* __restrict__ count,
+                       int H, __half* __restrict__ xc, int ldc, float* __restrict__ lsec, int* __restrict__ tc) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (i >= *count) return;
+  const int m = list[i];
+  const __half* src = x + static_cast<size_t>(m) * ldx;  // rows start on 16 bytes
+  __half* dst = xc + static_cast<size_t>(i) * ldc;
+  for (int c = lane * 8; c < H; c += 256) {
+    if (c + 8 <= H) {
+      *reinterpret_cast<uint4*>(dst + c) = __ldg(reinterpret_cast<const uint4*>(src + c));
+    } else {
+      for (int j = c; j < H; ++j) dst[j] = src[j];
+    }
+  }
+  if (lane == 0) {
+    lsec[i] = lse[m];
+    tc[i] = targets[m];
+  }
+}
+
 // dx row m from the K slices' partial sums (slab k: rows [k * slab_rows, ...)
 // of acc), in slice order, and the target's own term in fp32.
 __global__ void __launch_bounds__(256)
     logprob_dx_kernel(const float* __restrict__ acc, int slabs, int slab_rows, int ld_acc,
+                      const int* __restrict__ place,
                       const __half* __restrict__ x, int ldx, const __half* __restrict__ E, int lde,
                       const float* __restrict__ lse, const float* __restrict__ dlogp, const int* __restrict__ targets,
                       int H, int V, float scale, __half* __restrict__ dx, int lddx) {
@@ -152,17 +354,18 @@ __global__ void __launch_bounds__(256)
   }
   __syncthreads();
   pdl_wait();
+  const int at = place ? place[m] : m;  // the row of the partial sums; -1: it has no gradient
   // 1 - p_t without cancellation for a confident token
   const float g = ok ? scale * dlogp[m] : 0.f;
   const float one_minus = ok ? -expm1f(s_exact - lse[m]) : 0.f;
   const float unshift = exp2f(-kProbShift);
   const __half* et = E + static_cast<size_t>(ok ? t : 0) * lde;
-  const float* a0 = acc + static_cast<size_t>(m) * ld_acc;
+  const float* a0 = acc + static_cast<size_t>(max(at, 0)) * ld_acc;
   __half* out = dx + static_cast<size_t>(m) * lddx;
   const bool vec = (reinterpret_cast<uintptr_t>(dx) & 7) == 0 && (lddx & 3) == 0;
   for (int c = threadIdx.x * 4; c < H; c += blockDim.x * 4) {
     float r[4] = {0.f, 0.f, 0.f, 0.f};
-    if (ok) {
+    if (ok && at >= 0) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = 0; k < slabs; ++k) {  // ld_acc is a multiple of 4; what lies past H is not used
         const float4 o = *reinterpret_cast<const float4*>(a0 + static_cast<size_t>(k) * slab_rows * ld_acc + c);
@@ -230,6 +433,14 @@ BwdPlan bwd_plan(int M, int H, int V) {
   return p;
 }
 
+// More rows than one CTA pair's tile: the ones without a gradient (prompts,
+// padding, clipped tokens) are left out of both products.  The copy of the
+// others costs about 10 us of 4.5 ms at 4096 x 2048 x 151936.
+constexpr int kGatherRows = 256;
+
+// rows for the TMA and for 16-byte loads
+bool rows_ok(const __half* p, int ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
+
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct PdlScope {  // the chain's kernels await one another (pdl_wait); the first is launched normally
@@ -242,7 +453,10 @@ struct PdlScope {  // the chain's kernels await one another (pdl_wait); the firs
 size_t lm_logprobs_workspace(int M, int H, int V, bool backward) {
   if (!backward) return up256(sizeof(float) * M) + up256(sizeof(float2) * static_cast<size_t>(M) * ((V + 127) / 128));
   const BwdPlan p = bwd_plan(M, H, V);
-  return up256(sizeof(__half) * static_cast<size_t>(M) * p.vc) +
+  const size_t gather = M > kGatherRows ? 4 * up256(sizeof(int) * M) + 256 +
+                                              up256(sizeof(__half) * static_cast<size_t>(M) * ((H + 7) / 8 * 8))
+                                        : 0;
+  return gather + up256(sizeof(__half) * static_cast<size_t>(M) * p.vc) +
          up256(sizeof(float) * static_cast<size_t>(p.slabs) * p.slab_rows * p.ld_acc);
 }
 
@@ -255,14 +469,21 @@ cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, fl
 
 cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, float* logp, float* lse, int M, int H,
                         int V, int ldx, int lde, float2* part, float* tgt_logit, int* err, cudaStream_t st) {
-  const int slots = (V + 127) / 128;
+  int slots = (V + 127) / 128;
   EpiArgs ea;
   ea.targets = targets;
   ea.tgt_logit = tgt_logit;
   ea.part2 = part;
   PdlScope scope;
   set_pdl(false);
-  cudaError_t e = gemm(Operand{x, M, H, ldx}, Operand{E, V, H, lde}, M, V, Epi::kLogProb, ea, err, st, 256);
+  cudaError_t e;
+  if (!rows_ok(x, ldx) || !rows_ok(E, lde)) return cudaErrorInvalidValue;
+  if (M <= kFewRows && sizeof(float) * kFewRows * (H + 255) <= kFewSmem) {
+    slots = std::min(slots, kFewBlocks * gemm_num_sms());
+    e = (M == 1 ? few_rows<1> : few_rows<2>)(x, E, targets, M, H, V, ldx, lde, part, tgt_logit, slots, st);
+  } else {
+    e = gemm(Operand{x, M, H, ldx}, Operand{E, V, H, lde}, M, V, Epi::kLogProb, ea, err, st, 256);
+  }
   if (e != cudaSuccess) return e;
   set_pdl(true);
   return launch_pdl(logprob_finish_kernel, (M + kRows - 1) / kRows, kRows * kWarps, 0, st, ea.part2, ea.tgt_logit,
@@ -272,22 +493,52 @@ cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, fl
 cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* targets, const float* lse,
                                  const float* dlogp, __half* dx, int M, int H, int V, int ldx, int lde, int lddx,
                                  float scale, void* ws, int* err, cudaStream_t st) {
+  if (!rows_ok(x, ldx) || !rows_ok(E, lde)) return cudaErrorInvalidValue;
   const BwdPlan p = bwd_plan(M, H, V);
   char* w = static_cast<char*>(ws);
   __half* pc = reinterpret_cast<__half*>(w);
   float* acc = reinterpret_cast<float*>(w + up256(sizeof(__half) * static_cast<size_t>(M) * p.vc));
   PdlScope scope;
   set_pdl(false);
+  const int* in_targets = targets;
+  const float* in_lse = lse;
+  const __half* in_x = x;
+  const int* m_rows = nullptr;
+  const int* place = nullptr;
+  int in_ldx = ldx;
+  if (M > kGatherRows) {
+    char* g = reinterpret_cast<char*>(acc) + up256(sizeof(float) * static_cast<size_t>(p.slabs) * p.slab_rows * p.ld_acc);
+    const size_t ints = up256(sizeof(int) * M);
+    int* list = reinterpret_cast<int*>(g);
+    int* at = reinterpret_cast<int*>(g + ints);
+    int* tc = reinterpret_cast<int*>(g + 2 * ints);
+    float* lsec = reinterpret_cast<float*>(g + 3 * ints);
+    int* count = reinterpret_cast<int*>(g + 4 * ints);
+    __half* xc = reinterpret_cast<__half*>(g + 4 * ints + 256);
+    in_ldx = (H + 7) / 8 * 8;
+    cudaError_t e = launch_pdl(live_rows_kernel, 1, 1024, 0, st, targets, dlogp, M, V, list, at, count);
+    if (e != cudaSuccess) return e;
+    set_pdl(true);
+    e = launch_pdl(gather_rows_kernel, (M + 7) / 8, 256, 0, st, x, ldx, lse, targets, list, count, H, xc, in_ldx, lsec,
+                   tc);
+    if (e != cudaSuccess) return e;
+    in_targets = tc;
+    in_lse = lsec;
+    in_x = xc;
+    m_rows = count;
+    place = at;
+  }
   for (int v0 = 0; v0 < V; v0 += p.vc) {
     const int n = std::min(p.vc, V - v0);
     const __half* Ec = E + static_cast<size_t>(v0) * lde;
     EpiArgs ea;
-    ea.targets = targets;
-    ea.lse = lse;
+    ea.targets = in_targets;
+    ea.lse = in_lse;
+    ea.m_rows = m_rows;
     ea.vocab_off = v0;
     ea.out = pc;
     ea.ld_out = p.vc;
-    cudaError_t e = gemm(Operand{x, M, H, ldx}, Operand{Ec, n, H, lde}, M, n, Epi::kProbs, ea, err, st, 256);
+    cudaError_t e = gemm(Operand{in_x, M, H, in_ldx}, Operand{Ec, n, H, lde}, M, n, Epi::kProbs, ea, err, st, 256);
     if (e != cudaSuccess) return e;
     set_pdl(true);
     EpiArgs eb;
@@ -296,11 +547,12 @@ cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* ta
     eb.accumulate = v0 > 0;
     eb.ksplit = p.slabs;
     eb.slab_rows = p.slab_rows;
+    eb.m_rows = m_rows;
     // acc (+)= probabilities . E_c (E_c [n, H] read MN-major); one writer per element and chunk
     e = gemm(Operand{pc, M, n, p.vc}, Operand{Ec, H, n, lde, true}, M, H, Epi::kStoreF32, eb, err, st, 256);
     if (e != cudaSuccess) return e;
   }
-  return launch_pdl(logprob_dx_kernel, M, 256, 0, st, acc, p.slabs, p.slab_rows, p.ld_acc, x, ldx, E, lde, lse,
+  return launch_pdl(logprob_dx_kernel, M, 256, 0, st, acc, p.slabs, p.slab_rows, p.ld_acc, place, x, ldx, E, lde, lse,
                     dlogp, targets, H, V, scale, dx, lddx);
 }
 

@@ -136,6 +136,33 @@ def test_lm_logprobs_full_vocabulary(llmcu, cuda_device):
     assert (dx[11] == 0).all()
 
 
+@pytest.mark.parametrize("M", [1, 2, 257, 1500])
+@pytest.mark.parametrize("live", [0, 1, 0.03, 0.5])
+def test_lm_logprobs_backward_rows_without_gradient(llmcu, cuda_device, M, live):
+    """Rows whose upstream gradient is 0 or whose target scores nothing get zeros
+    and leave the others' bits alone, from none of the rows to one and half of them."""
+    H, V = 136, 5000
+    x, E, t = lm_case(cuda_device, M, H, V, 6)
+    logp, lse = lm_forward(llmcu, x, E, t)
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    dlogp = torch.randn(M, generator=g, device=cuda_device)
+    full = lm_backward(llmcu, x, E, t, lse, dlogp, 16.0)
+    on = torch.rand(M, generator=g, device=cuda_device) < live if isinstance(live, float) else torch.zeros(
+        M, dtype=torch.bool, device=cuda_device)
+    if live == 1:
+        on[M // 2] = True
+    off = ~on
+    half = torch.rand(M, generator=g, device=cuda_device) < 0.5
+    t2 = torch.where(off & half, -100, t)
+    d2 = torch.where(off & ~half, torch.zeros_like(dlogp), dlogp)
+    d2 = torch.where(off & half, float("nan"), d2)
+    got = lm_backward(llmcu, x, E, t2, lse, d2, 16.0)
+    assert (got[off] == 0).all()
+    # rows land in other tiles: the tensor cores' sums over K do not depend on the row
+    assert torch.equal(got[on], full[on])
+    assert llmcu.kernel_checks(stream()) == 0
+
+
 def test_lm_logprobs_gradient_by_differences(llmcu, cuda_device):
     """Central differences of the forward along random directions.  A direction d
     of unit length moved by h = 1/8: the third derivative of logp along d is at

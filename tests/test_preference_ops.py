@@ -39,6 +39,11 @@ def test_lm_logprobs_refusals(llmcu, backward):
     refused(llmcu, INVALID, lambda: lm(llmcu, backward, nbytes=size - 1))
     refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, ws=P + 16))
     refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, targets=P + 2))
+    # rows that the TMA cannot read
+    refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, x=P + 8))
+    refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, E=P + 2))
+    refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, ldx=68))
+    refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, lde=65))
     if backward:
         refused(llmcu, INVALID, lambda: lm(llmcu, backward, lddx=8))
         refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, dx=P + 1))
