@@ -341,7 +341,7 @@ struct PolicyArgs {
   // set by policy_loss
   float f_low, f_high, f_dual;  // the logarithms in fp32
   float near;                   // distance to one of them that fp32 does not resolve
-  bool vec;
+  bool vec, vec16;
   int row_quads;
   int64_t units;
   uint32_t div_m;

@@ -108,15 +108,22 @@ __device__ __forceinline__ void load4(const float* __restrict__ p, int64_t i, in
     for (int j = 0; j < 4; ++j) v[j] = i + j >= first && i + j < end ? __ldg(p + i + j) : fill;
   }
 }
+// The top bit of every byte of w that is not 0.
+__device__ __forceinline__ uint32_t nonzero_bytes(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) & 0x80808080u;
+}
+// Bit j: byte j of an aligned four is not 0 (the bits, 8 apart, brought together
+// by a product that carries none of them into another).
+__device__ __forceinline__ uint32_t mask4(const uint8_t* p) {
+  return ((nonzero_bytes(__ldg(reinterpret_cast<const uint32_t*>(p))) >> 7) * 0x01020408u) >> 24;
+}
 // Bit j: token i + j is scored (inside the row, and unmasked; no mask: all are).
 __device__ __forceinline__ uint32_t load_mask(const uint8_t* __restrict__ p, int64_t i, int64_t first, int64_t end,
                                               bool vec) {
   uint32_t b = 0;
   if (vec && i >= first && i + 4 <= end) {
     if (!p) return 15u;
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p + i));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) b |= ((w >> (8 * j)) & 0xffu) ? 1u << j : 0u;
+    b = mask4(p + i);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -312,18 +319,72 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyArgs& a, float l
   return t;
 }
 
+// Unit u: four places of a row, of which the row's tokens are set in `in`
+// (none: the unit lies past its row, or past the last).
+struct PolicyUnit {
+  int row;
+  uint32_t in;
+  int64_t i;
+  __device__ __forceinline__ PolicyUnit(const PolicyArgs& a, int64_t u) {
+    row = static_cast<int>(__umulhi(static_cast<uint32_t>(u), a.div_m) >> a.div_s);
+    const int64_t first = static_cast<int64_t>(row) * a.ld;
+    const int head = static_cast<int>(first) & 3;
+    const int c = 4 * (static_cast<int>(u) - row * a.row_quads) - head;  // column of the first place
+    i = first + c;
+    const int left = a.seq - c;
+    in = c < 0 ? 15u << -c : 15u;
+    if (left < 4) in = left > 0 ? in & ((1u << left) - 1u) : 0u;
+    in &= u < a.units ? 15u : 0u;
+  }
+  __device__ __forceinline__ bool whole(const PolicyArgs& a) const { return in == 15u && a.vec; }
+  // which of them are scored
+  __device__ __forceinline__ uint32_t mask(const PolicyArgs& a) const {
+    if (!a.mask) return in;
+    if (whole(a)) return mask4(a.mask + i);
+    uint32_t b = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if ((in >> j) & 1) b |= __ldg(a.mask + i + j) ? 1u << j : 0u;
+    return b;
+  }
+  __device__ __forceinline__ void store(const PolicyArgs& a, const float (&v)[4]) const {
+    if (whole(a)) {
+      *reinterpret_cast<float4*>(a.dlogp + i) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((in >> j) & 1) a.dlogp[i + j] = v[j];
+    }
+  }
+};
+
 // The four tokens of a quad: gradients (0 where nothing is scored), sums.
 struct PolicyQuad {
   float lp[4], old[4], adv[4], ref[4];
-  __device__ __forceinline__ void load(const PolicyArgs& a, int row, int64_t i, int64_t first, int64_t end) {
-    load4(a.logp, i, first, end, a.vec, 0.f, lp);
-    load4(a.old, i, first, end, a.vec, 0.f, old);
-    if (a.token_adv) {
-      load4(a.adv, i, first, end, a.vec, 0.f, adv);
+  __device__ __forceinline__ void load(const PolicyArgs& a, const PolicyUnit& p) {
+    if (!a.token_adv) adv[0] = adv[1] = adv[2] = adv[3] = __ldg(a.adv + p.row);
+    if (p.whole(a)) {
+      vec4(a.logp + p.i, lp);
+      vec4(a.old + p.i, old);
+      if (a.token_adv) vec4(a.adv + p.i, adv);
+      if (a.ref) vec4(a.ref + p.i, ref);
     } else {
-      adv[0] = adv[1] = adv[2] = adv[3] = __ldg(a.adv + row);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((p.in >> j) & 1) {
+          lp[j] = __ldg(a.logp + p.i + j);
+          old[j] = __ldg(a.old + p.i + j);
+          if (a.token_adv) adv[j] = __ldg(a.adv + p.i + j);
+          if (a.ref) ref[j] = __ldg(a.ref + p.i + j);
+        }
     }
-    if (a.ref) load4(a.ref, i, first, end, a.vec, 0.f, ref);
+  }
+  static __device__ __forceinline__ void vec4(const float* p, float (&v)[4]) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(p));
+    v[0] = x.x;
+    v[1] = x.y;
+    v[2] = x.z;
+    v[3] = x.w;
   }
   __device__ __forceinline__ void run(const PolicyArgs& a, uint32_t bits, float weight, float (&g)[4], float& loss,
                                       float& kl, int& clips) const {
@@ -336,24 +397,6 @@ struct PolicyQuad {
       kl += on ? t.kl : 0.f;
       clips += on && t.clip;
     }
-  }
-};
-
-// Row, first element and row's ends of unit u.
-struct PolicyUnit {
-  int row;
-  bool any;  // the unit holds tokens of its row
-  int64_t i, first, end;
-  __device__ __forceinline__ PolicyUnit(const PolicyArgs& a, int64_t u) {
-    row = static_cast<int>(__umulhi(static_cast<uint32_t>(u), a.div_m) >> a.div_s);
-    const int q = static_cast<int>(u) - row * a.row_quads;
-    first = static_cast<int64_t>(row) * a.ld;
-    end = first + a.seq;
-    i = (first & ~int64_t{3}) + 4 * q;
-    any = u < a.units && i < end;
-  }
-  __device__ __forceinline__ uint32_t mask(const PolicyArgs& a) const {
-    return any ? load_mask(a.mask, i, first, end, a.vec) : 0u;
   }
 };
 
@@ -390,7 +433,7 @@ __global__ void __launch_bounds__(kSmallThreads) policy_small_kernel(PolicyArgs 
   const PolicyUnit p(a, rank * nt + threadIdx.x);
   const uint32_t bits = p.mask(a);
   PolicyQuad quad;
-  if (p.any) quad.load(a, p.row, p.i, p.first, p.end);
+  if (bits) quad.load(a, p);
   if (by_row && bits) atomicAdd(&rows[p.row], __popc(bits));
   float weight = a.inv_norm;
   if (a.agg == kPolicyTokenMean) {
@@ -416,12 +459,27 @@ __global__ void __launch_bounds__(kSmallThreads) policy_small_kernel(PolicyArgs 
   float g[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, kl = 0.f;
   int clips = 0;
   if (bits) quad.run(a, bits, weight, g, l, kl, clips);
-  if (a.dlogp && p.any) store4(a.dlogp, p.i, p.first, p.end, a.vec, g);
+  if (a.dlogp) p.store(a, g);
   double v[4] = {static_cast<double>(l * weight), static_cast<double>(kl), static_cast<double>(clips),
                  static_cast<double>(__popc(bits))};
   block_sums(v, red);
   cluster_sums(v, slots[1], C, rank, a.agg == kPolicyConstant, false);
   if (rank == 0 && threadIdx.x == 0) write_stats(v, a.stats);
+}
+
+// Scored tokens among the 16 mask bytes from index i (a multiple of 16) on,
+// inside [first, end).
+__device__ __forceinline__ int count16(const PolicyArgs& a, int64_t i, int64_t first, int64_t end) {
+  if (!a.mask) return static_cast<int>(min(i + 16, end) - max(i, first));
+  int n = 0;
+  if (a.vec16 && i >= first && i + 16 <= end) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(a.mask + i));
+    n = __popc(nonzero_bytes(w.x)) + __popc(nonzero_bytes(w.y)) + __popc(nonzero_bytes(w.z)) +
+        __popc(nonzero_bytes(w.w));
+  } else {
+    for (int64_t j = max(i, first); j < min(i + 16, end); ++j) n += __ldg(a.mask + j) != 0;
+  }
+  return n;
 }
 
 // Scored tokens: of each row (one CTA or warp a row) into counts[row], or of
@@ -430,26 +488,30 @@ __global__ void __launch_bounds__(kThreads) policy_count_kernel(PolicyArgs a, in
   pdl_trigger();
   __shared__ int red[kThreads / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int n = 0;
+  auto count_row = [&](int row, int at, int step) {
+    const int64_t first = static_cast<int64_t>(row) * a.ld, end = first + a.seq;
+    for (int64_t i = (first & ~int64_t{15}) + 16 * at; i < end; i += 16 * step) n += count16(a, i, first, end);
+  };
   if (a.agg == kPolicySequenceMean && a.seq <= 1024) {  // a warp a row
     const int row = blockIdx.x * (kThreads / 32) + w;
-    if (row >= a.batch) return;
-    const RowSpan r(row, a.ld, a.seq);
-    int n = 0;
-    for (int q = lane; q < r.nq; q += 32) n += __popc(load_mask(a.mask, (r.q0 + q) << 2, r.first, r.end, a.vec));
+    if (row < a.batch) count_row(row, lane, 32);
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) counts[row] = n;
+    if (lane == 0 && row < a.batch) counts[row] = n;
     return;
   }
-  int n = 0;
   if (a.agg == kPolicySequenceMean) {  // a CTA a row
-    const RowSpan r(blockIdx.x, a.ld, a.seq);
-    for (int q = threadIdx.x; q < r.nq; q += kThreads)
-      n += __popc(load_mask(a.mask, (r.q0 + q) << 2, r.first, r.end, a.vec));
-  } else {
-    for (int64_t u = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; u < a.units;
-         u += static_cast<int64_t>(gridDim.x) * kThreads) {
-      const PolicyUnit p(a, u);
-      n += __popc(p.mask(a));
+    count_row(blockIdx.x, threadIdx.x, kThreads);
+  } else if (a.seq <= 2048) {  // warps take rows in turn
+    for (int row = blockIdx.x * (kThreads / 32) + w; row < a.batch; row += gridDim.x * (kThreads / 32))
+      count_row(row, lane, 32);
+  } else {  // the grid takes rows' pieces of 256 x 16 tokens in turn
+    const int pieces = (a.seq + 15 + 16 * kThreads - 1) / (16 * kThreads);
+    for (int64_t k = blockIdx.x; k < static_cast<int64_t>(a.batch) * pieces; k += gridDim.x) {
+      const int row = static_cast<int>(k / pieces);
+      const int64_t first = static_cast<int64_t>(row) * a.ld, end = first + a.seq;
+      const int64_t i = (first & ~int64_t{15}) + 16 * ((k - static_cast<int64_t>(row) * pieces) * kThreads + threadIdx.x);
+      if (i < end) n += count16(a, i, first, end);
     }
   }
   n = __reduce_add_sync(0xffffffffu, n);
@@ -476,20 +538,19 @@ __global__ void __launch_bounds__(kThreads, kMainBlocks)
   double v[4] = {0.0, 0.0, 0.0, 0.0};
   int clips = 0;
   int64_t tokens = 0;
-  // the mask of the next unit is fetched a turn ahead, so that the loads it
-  // decides on wait for nothing
-  // a CTA takes a run of units
+  // A CTA takes a run of units; the mask of the next one is fetched a turn
+  // ahead, so that the loads it decides on wait for nothing
   const int64_t run = (a.units + gridDim.x - 1) / gridDim.x;
   const int64_t u_end = min(a.units, (blockIdx.x + 1) * run);
   int64_t u = blockIdx.x * run + threadIdx.x;
-  PolicyUnit next(a, min(u, u_end));
-  uint32_t next_bits = u < u_end ? next.mask(a) : 0u;
+  PolicyUnit next(a, u < u_end ? u : a.units);
+  uint32_t next_bits = next.mask(a);
   for (; u < u_end; u += kThreads) {
     const PolicyUnit p = next;
     const uint32_t bits = next_bits;
     float g[4] = {0.f, 0.f, 0.f, 0.f};
     PolicyQuad quad;
-    if (bits) quad.load(a, p.row, p.i, p.first, p.end);
+    if (bits) quad.load(a, p);
     if (u + kThreads < u_end) {
       next = PolicyUnit(a, u + kThreads);
       next_bits = next.mask(a);
@@ -503,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, kMainBlocks)
       v[1] += static_cast<double>(kl);
       tokens += __popc(bits);
     }
-    if (a.dlogp && p.any) store4(a.dlogp, p.i, p.first, p.end, a.vec, g);
+    if (a.dlogp) p.store(a, g);
   }
   v[2] = static_cast<double>(clips);
   v[3] = static_cast<double>(tokens);
@@ -530,7 +591,7 @@ __global__ void __launch_bounds__(kThreads) policy_stats_kernel(const double* __
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-constexpr int kCountBlocks = 296;  // CTAs of the token count: two an SM
+constexpr int kCountBlocks = 1184;  // CTAs of the token count: eight an SM
 
 int policy_blocks(int64_t units) {
   const int64_t want = (units + kThreads - 1) / kThreads;
@@ -556,6 +617,7 @@ size_t policy_loss_workspace(int batch) {
 }
 
 cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
+  a.vec16 = aligned(a.mask, 16);
   a.vec = aligned(a.logp, 16) && aligned(a.old, 16) && aligned(a.ref, 16) && aligned(a.mask, 4) &&
           aligned(a.dlogp, 16) && (!a.token_adv || aligned(a.adv, 16));
   // unit u: quad u % row_quads of row u / row_quads (a row of seq tokens
@@ -594,7 +656,7 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
   if (a.agg == kPolicySequenceMean) {
     n_counts = a.seq <= 1024 ? (a.batch + kThreads / 32 - 1) / (kThreads / 32) : a.batch;
   } else if (a.agg == kPolicyTokenMean) {
-    n_counts = static_cast<int>(std::min<int64_t>(kCountBlocks, (a.units + kThreads - 1) / kThreads));
+    n_counts = static_cast<int>(std::min<int64_t>(kCountBlocks, (a.units / 4 + kThreads - 1) / kThreads + 1));
   }
   if (n_counts) {
     e = launch_pdl(policy_count_kernel, n_counts, kThreads, 0, st, a, counts);
