@@ -58,22 +58,30 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
-// Launch `kern` in clusters of C CTAs (grid: a multiple of C).
+// Launch `kern` in clusters of C CTAs (grid: a multiple of C), with programmatic
+// stream serialization if `chained`.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_cluster(void (*kern)(KArgs...), unsigned grid, int block, int C, size_t smem, cudaStream_t st,
-                                  Args... args) {
+                                  bool chained, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (C > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = C;
+    at[n].val.clusterDim.y = 1;
+    at[n++].val.clusterDim.z = 1;
+  }
+  if (chained) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = C > 1 ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
@@ -370,6 +378,7 @@ struct MuonArgs {
   int nesterov, match_rms, steps;
   // set by muon_update
   int cluster, tile, pitch;
+  bool chained;  // not the first of its launches
 };
 cudaError_t muon_update(MuonArgs a, cudaStream_t st);
 

@@ -608,7 +608,7 @@ cudaError_t preference_loss(PreferenceArgs a, cudaStream_t st) {
   const int quads = a.seq / 4 + 2;
   while (C < 8 && quads > 4 * C * kThreads && static_cast<int64_t>(a.pairs) * C < 8LL * gemm_num_sms()) C *= 2;
   a.cluster = C;
-  return launch_cluster(preference_kernel, static_cast<unsigned>(a.pairs) * C, kThreads, C, 0, st, a);
+  return launch_cluster(preference_kernel, static_cast<unsigned>(a.pairs) * C, kThreads, C, 0, st, false, a);
 }
 
 size_t policy_loss_workspace(int batch) {
@@ -645,7 +645,7 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
     int C = 1;
     while (C * nt < a.units) C *= 2;
     const size_t smem = a.agg == kPolicySequenceMean ? sizeof(int) * C * a.batch : 0;
-    return launch_cluster(policy_small_kernel, C, nt, C, smem, st, a, C);
+    return launch_cluster(policy_small_kernel, C, nt, C, smem, st, false, a, C);
   }
   double* partial = static_cast<double*>(ws);
   int* counts = reinterpret_cast<int*>(partial + 4 * kMainBlocks * static_cast<size_t>(gemm_num_sms()));
