@@ -410,9 +410,10 @@ llmcu_status llmcu_attention_bwd_noalloc(const void* q, const void* k, const voi
  * bounded wait that gave up is reported by llmcu_kernel_checks.  They may be
  * captured into a CUDA graph.  Calls that may run at the same time need
  * workspaces of their own; a workspace needs no initial contents and must be
- * 256-byte aligned (LLMCU_ERR_UNSUPPORTED otherwise).  Sums run in a fixed
- * order: the same call gives the same bits.  No reference counterpart: the
- * reference trains with the cross-entropy and AdamW only. */
+ * 256-byte aligned (LLMCU_ERR_UNSUPPORTED otherwise).  Outputs must not overlap
+ * inputs or the workspace (the Muon update works in place on w and momentum).
+ * Sums run in a fixed order: the same call gives the same bits.  No reference
+ * counterpart: the reference trains with the cross-entropy and AdamW only. */
 
 /* Token log-probabilities of hidden states under a tied head, without logits
  * in memory: logp[m] = x[m] . E[t] - lse[m] with t = targets[m] and lse[m] =
@@ -421,7 +422,9 @@ llmcu_status llmcu_attention_bwd_noalloc(const void* q, const void* k, const voi
  * the TMA needs, else LLMCU_ERR_UNSUPPORTED); targets int32 [rows]; logp and
  * lse fp32 [rows].  A target outside [0, vocab) scores nothing: logp is 0 (lse
  * is the row's all the same).  `workspace` has at least
- * llmcu_lm_logprobs_workspace(rows, hidden, vocab, 0) bytes. */
+ * llmcu_lm_logprobs_workspace(rows, hidden, vocab, 0) bytes (0 for sizes that
+ * are refused).  At most 2^24 rows, 2^20 columns of x and 2^30 of the vocabulary
+ * (LLMCU_ERR_UNSUPPORTED). */
 size_t llmcu_lm_logprobs_workspace(int rows, int hidden, int vocab, int backward);
 llmcu_status llmcu_lm_logprobs(const void* x, const void* E, const int32_t* targets, float* logp, float* lse,
                                int rows, int hidden, int vocab, int ldx, int lde, void* workspace,
@@ -458,8 +461,8 @@ typedef struct {
  * loss [pairs], reward [2 * pairs] (beta * R) and dlogp [2 * pairs, seq] are
  * fp32 outputs, each nullable.  dlogp is the gradient of sum_i dloss[i] *
  * loss[i]; dloss fp32 [pairs], null = 1 / pairs (the mean loss).  It is 0 where
- * nothing is scored; columns from seq to ld are left as they are.  Outputs must
- * not overlap inputs. */
+ * nothing is scored; columns from seq to ld are left as they are.  At most 2^27
+ * pairs and 2^30 tokens a row (LLMCU_ERR_UNSUPPORTED). */
 llmcu_status llmcu_preference_loss(const llmcu_preference_cfg* cfg, const float* logp, const float* ref_logp,
                                    const uint8_t* mask, const float* dloss, float* loss, float* reward, float* dlogp,
                                    int pairs, int seq, int ld, void* stream);
@@ -488,8 +491,8 @@ size_t llmcu_policy_loss_workspace(int batch, int seq);
  * (no KL term), mask as above.  stats (4 floats) receives the loss, the mean
  * of e^d - d - 1 over the scored tokens, the share of them that clip, and their
  * number (exact to 2^24); dlogp (nullable) the loss's gradient, 0 where nothing
- * is scored.  batch * max(2, (seq + 6) / 4) must stay below 2^31
- * (LLMCU_ERR_UNSUPPORTED). */
+ * is scored; columns from seq to ld are left as they are.  seq is at most 2^30
+ * and batch * max(2, (seq + 6) / 4) below 2^31 (LLMCU_ERR_UNSUPPORTED). */
 llmcu_status llmcu_policy_loss(const llmcu_policy_cfg* cfg, const float* logp, const float* old_logp,
                                const float* ref_logp, const float* advantages, const uint8_t* mask, float* stats,
                                float* dlogp, int batch, int seq, int ld, void* workspace, size_t workspace_bytes,

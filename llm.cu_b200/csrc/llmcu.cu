@@ -2228,8 +2228,14 @@ llmcu_status llmcu_attention_bwd(const void* q, const void* k, const void* v, co
 
 // ------------------------------------------------------ preference tuning
 
+// sizes whose sums and tile counts stay inside 32 bits
+constexpr int kMaxRows = 1 << 24, kMaxLen = 1 << 30;
+static bool lm_too_large(int rows, int hidden, int vocab) {
+  return rows > kMaxRows || hidden > (1 << 20) || vocab > kMaxLen;
+}
+
 size_t llmcu_lm_logprobs_workspace(int rows, int hidden, int vocab, int backward) {
-  if (rows <= 0 || hidden <= 0 || vocab <= 0) return 0;
+  if (rows <= 0 || hidden <= 0 || vocab <= 0 || lm_too_large(rows, hidden, vocab)) return 0;
   return lm_logprobs_workspace(rows, hidden, vocab, backward != 0);
 }
 
@@ -2245,6 +2251,7 @@ static bool bad_floats(std::initializer_list<const void*> ps) {
 llmcu_status llmcu_lm_logprobs(const void* x, const void* E, const int32_t* targets, float* logp, float* lse, int rows,
                                int hidden, int vocab, int ldx, int lde, void* workspace, size_t workspace_bytes,
                                void* stream) {
+  if (lm_too_large(rows, hidden, vocab)) return LLMCU_ERR_UNSUPPORTED;
   if (!x || !E || !targets || !logp || !lse || !workspace || rows <= 0 || hidden <= 0 || vocab <= 0 || ldx < hidden ||
       lde < hidden || workspace_bytes < lm_logprobs_workspace(rows, hidden, vocab, false))
     return LLMCU_ERR_INVALID_ARG;
@@ -2260,6 +2267,7 @@ llmcu_status llmcu_lm_logprobs(const void* x, const void* E, const int32_t* targ
 llmcu_status llmcu_lm_logprobs_bwd(const void* x, const void* E, const int32_t* targets, const float* lse,
                                    const float* dlogp, void* dx, int rows, int hidden, int vocab, int ldx, int lde,
                                    int lddx, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  if (lm_too_large(rows, hidden, vocab)) return LLMCU_ERR_UNSUPPORTED;
   if (!x || !E || !targets || !lse || !dlogp || !dx || !workspace || rows <= 0 || hidden <= 0 || vocab <= 0 ||
       ldx < hidden || lde < hidden || lddx < hidden ||
       workspace_bytes < lm_logprobs_workspace(rows, hidden, vocab, true))
@@ -2278,8 +2286,8 @@ llmcu_status llmcu_preference_loss(const llmcu_preference_cfg* cfg, const float*
                                    const uint8_t* mask, const float* dloss, float* loss, float* reward, float* dlogp,
                                    int pairs, int seq, int ld, void* stream) {
   PreferenceArgs a{};
-  if (!preference_args(cfg, &a) || !logp || pairs <= 0 || pairs > (1 << 27) || seq <= 0 || ld < seq)
-    return LLMCU_ERR_INVALID_ARG;
+  if (!preference_args(cfg, &a) || !logp || pairs <= 0 || seq <= 0 || ld < seq) return LLMCU_ERR_INVALID_ARG;
+  if (pairs > (1 << 27) || seq > kMaxLen) return LLMCU_ERR_UNSUPPORTED;
   if (bad_floats({logp, ref_logp, dloss, loss, reward, dlogp})) return LLMCU_ERR_UNSUPPORTED;
   a.logp = logp;
   a.ref = ref_logp;
@@ -2306,6 +2314,7 @@ llmcu_status llmcu_policy_loss(const llmcu_policy_cfg* cfg, const float* logp, c
   if (!policy_args(cfg, &a) || !logp || !old_logp || !advantages || !stats || !workspace || batch <= 0 || seq <= 0 ||
       ld < seq || workspace_bytes < policy_loss_workspace(batch))
     return LLMCU_ERR_INVALID_ARG;
+  if (seq > kMaxLen) return LLMCU_ERR_UNSUPPORTED;
   if (bad_workspace(workspace) || bad_floats({logp, old_logp, ref_logp, advantages, stats, dlogp}))
     return LLMCU_ERR_UNSUPPORTED;
   a.logp = logp;
@@ -2326,7 +2335,7 @@ llmcu_status llmcu_muon_update(const llmcu_muon_cfg* cfg, float* w, const float*
   MuonArgs a{};
   if (!muon_args(cfg, &a) || !w || !grad || !momentum || count <= 0 || rows <= 0 || cols <= 0)
     return LLMCU_ERR_INVALID_ARG;
-  if (bad_floats({w, grad, momentum})) return LLMCU_ERR_UNSUPPORTED;
+  if (bad_floats({w, grad, momentum}) || rows > kMaxLen || cols > kMaxLen) return LLMCU_ERR_UNSUPPORTED;
   a.w = w;
   a.grad = grad;
   a.mom = momentum;

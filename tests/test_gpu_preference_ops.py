@@ -350,6 +350,28 @@ def test_preference_offsets_past_32_bits(llmcu, cuda_device):
     assert torch.allclose(dl[:, :S], want[2], rtol=4 * U, atol=0)
 
 
+@pytest.mark.parametrize("agg", [0, 1, 2])
+def test_policy_offsets_past_32_bits(llmcu, cuda_device, agg):
+    """Three rows 1.1 billion elements apart (too many tokens for the one-launch kernel in the second half)."""
+    B, ld = 3, 1_100_000_001
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GB of free device memory")
+    lp, old, dl = (torch.empty(B, ld, device=cuda_device) for _ in range(3))
+    mask = torch.empty(B, ld, dtype=torch.uint8, device=cuda_device)
+    for S in (9, 12001):
+        small = policy_inputs(cuda_device, B, S, S, 8, False)
+        lp[:, :S], old[:, :S], mask[:, :S] = small[0], small[1], small[4].to(torch.uint8)
+        cfg = llmcu.Policy(agg=agg, norm=50.0)
+        n = llmcu.policy_loss_workspace(B, S)
+        ws, stats = torch.empty(n, dtype=torch.uint8, device=cuda_device), torch.empty(4, device=cuda_device)
+        llmcu.policy_loss(cfg, lp.data_ptr(), old.data_ptr(), 0, small[3].data_ptr(), mask.data_ptr(),
+                          stats.data_ptr(), dl.data_ptr(), B, S, ld, ws.data_ptr(), n, stream())
+        want = run_policy(llmcu, cfg, small[0], small[1], None, small[3], small[4], B, S, S, cuda_device)
+        # the quads fall otherwise, and with them the order of the sums of up to four fp32 terms
+        assert torch.equal(dl[:, :S], want[1])
+        assert torch.allclose(stats, want[0], rtol=1e-5, atol=1e-6)
+
+
 # ----------------------------------------------------------------- policy loss
 def policy_inputs(dev, B, S, ld, seed, token_adv, empty=()):
     g = torch.Generator(device=dev).manual_seed(seed)

@@ -49,6 +49,25 @@ def test_lm_logprobs_refusals(llmcu, backward):
         refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, dx=P + 1))
 
 
+BIG = (1 << 31) - 1
+
+
+def test_sizes_past_32_bits_are_refused(llmcu):
+    """The largest ints a caller can pass are turned down, not wrapped around."""
+    for kw in (dict(rows=BIG), dict(rows=(1 << 24) + 1), dict(hidden=BIG, ldx=BIG, lde=BIG, lddx=BIG),
+               dict(vocab=BIG)):
+        for backward in (False, True):
+            refused(llmcu, UNSUPPORTED, lambda: lm(llmcu, backward, nbytes=1 << 60, **kw))
+    assert llmcu.lm_logprobs_workspace(BIG, 64, 512) == 0 and llmcu.lm_logprobs_workspace(4, 64, BIG, True) == 0
+    refused(llmcu, UNSUPPORTED, lambda: llmcu.preference_loss(llmcu.Preference(), P, 0, 0, 0, P, P, P, 1, BIG, BIG))
+    refused(llmcu, UNSUPPORTED, lambda: llmcu.preference_loss(llmcu.Preference(), P, 0, 0, 0, P, P, P, BIG, 1, 1))
+    refused(llmcu, UNSUPPORTED, lambda: llmcu.policy_loss(llmcu.Policy(), P, P, 0, P, 0, P, P, 1, BIG, BIG, P, 1 << 30))
+    refused(llmcu, UNSUPPORTED, lambda: llmcu.policy_loss(llmcu.Policy(), P, P, 0, P, 0, P, P, 1 << 30, 1, 1, P,
+                                                          1 << 40))
+    refused(llmcu, UNSUPPORTED, lambda: llmcu.muon_update(llmcu.Muon(), P, P, P, 1, 16, BIG))
+    refused(llmcu, UNSUPPORTED, lambda: llmcu.muon_update(llmcu.Muon(), P, P, P, 1, BIG, BIG))
+
+
 def test_workspace_sizes(llmcu):
     assert llmcu.lm_logprobs_workspace(0, 64, 512) == 0 and llmcu.lm_logprobs_workspace(4, 64, -1, True) == 0
     assert llmcu.lm_logprobs_workspace(1, 2048, 151936) >= 4 + 8 * 1187
