@@ -209,17 +209,13 @@ __global__ void __launch_bounds__(kRows* kWarps)
                           int M, int H, int V, int ldx, int lde, int slots, float* __restrict__ logp,
                           float* __restrict__ lse) {
   pdl_trigger();
-  __shared__ float2 red[kWarps][kRows];
-  __shared__ float exact[kRows];
+  __shared__ float2 red[kWarps][kRows + 1];  // + 1: read down its columns
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  {
-    const int row = blockIdx.x * kRows + w;
-    const int t = row < M ? targets[row] : -1;
-    if (t >= 0 && t < V) {
-      const float l = target_logit(x + static_cast<size_t>(row) * ldx, E + static_cast<size_t>(t) * lde, H, lane);
-      if (lane == 0) exact[w] = l;
-    }
-  }
+  const int row = blockIdx.x * kRows + w;
+  const int t = row < M ? targets[row] : -1;
+  const bool ok = t >= 0 && t < V;
+  float exact = 0.f;
+  if (ok) exact = target_logit(x + static_cast<size_t>(row) * ldx, E + static_cast<size_t>(t) * lde, H, lane);
   pdl_wait();
   const int m = blockIdx.x * kRows + lane;
   float2 p = make_float2(-INFINITY, 0.f);
@@ -229,20 +225,20 @@ __global__ void __launch_bounds__(kRows* kWarps)
   }
   red[w][lane] = p;
   __syncthreads();
-  if (w == 0 && m < M) {
-    p = red[0][lane];
-    for (int i = 1; i < kWarps; ++i) p = join_pairs(p, red[i][lane]);
-    const float mx = p.x;
+  if (row >= M) return;
+  p = red[lane][w];  // the 32 parts of row w
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    p = join_pairs(p, make_float2(__shfl_xor_sync(0xffffffffu, p.x, o), __shfl_xor_sync(0xffffffffu, p.y, o)));
+  if (lane == 0) {
     float s = p.y;
-    const int t = targets[m];
-    const bool ok = t >= 0 && t < V;
     if (ok) {
-      const float rough = tgt_logit[m], d = exact[lane] - rough;
-      if (isfinite(d)) s = fmaf(exp2f((rough - mx) * kLog2e), expm1f(d), s);
+      const float rough = tgt_logit[row], d = exact - rough;
+      if (isfinite(d)) s = fmaf(exp2f((rough - p.x) * kLog2e), expm1f(d), s);
     }
-    const float l = mx + logf(s);
-    lse[m] = l;
-    logp[m] = ok ? exact[lane] - l : 0.f;
+    const float l = p.x + logf(s);
+    lse[row] = l;
+    logp[row] = ok ? exact - l : 0.f;
   }
 }
 
