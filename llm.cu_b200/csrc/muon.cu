@@ -71,48 +71,68 @@ __device__ __forceinline__ void small_product(const double* A, const double* B, 
   d[1] += d2[1];
 }
 
-struct Tile {
+// 32 columns of a matrix (fewer at its end), which one warp takes through every
+// step: loading, G, the product with P and the update of w, without a word to
+// the other warps, so that the warps' loads and products overlap.
+constexpr int kCols = 32;
+constexpr int kScalar = 4;  // single elements a lane loads at once
+struct Chunk {
+  int64_t base;  // its first element in the buffers
+  int64_t row;   // wide: elements between rows
+  float* u;      // its first column in shared memory, rows `pitch` apart
   int pitch;
-  int k, len;      // rows, columns of this tile
-  int64_t base;    // the tile's first element in the buffers
-  int64_t row;     // wide: elements between rows
+  int k, len;    // rows, columns
   bool tall, vec;
-  uint32_t inv;    // ceil(2^32 / d) of the division below; 0 for d = 1
-  int d;           // wide: groups of a row; tall: k
+  uint32_t inv;  // ceil(2^32 / k) for the tall layout's divisions; 0 for k = 1
 
-  // Elements in memory order, in groups of four (vec) or single ones.
-  __device__ __forceinline__ int groups() const {
-    if (tall) return vec ? (k * len) >> 2 : k * len;
-    return k * d;
-  }
-  __device__ __forceinline__ void divisor(int n) {
-    d = n;
-    inv = n > 1 ? 0xffffffffu / static_cast<uint32_t>(n) + 1u : 0u;
-  }
-  // x / d for x < 2^32 / d: a tile has at most 16 * kMaxTile elements
-  __device__ __forceinline__ int div(int x) const {
+  // x / k for x < 512
+  __device__ __forceinline__ int div_k(int x) const {
     return inv ? static_cast<int>(__umulhi(static_cast<uint32_t>(x), inv)) : x;
   }
-  __device__ __forceinline__ int64_t offset(int e) const {
-    if (tall) return base + (vec ? 4 * e : e);
-    const int r = div(e);
-    return base + r * row + (e - r * d) * (vec ? 4 : 1);
+  // vec: group e < 8 k is four elements that lie together in memory
+  __device__ __forceinline__ int64_t offset4(int e) const {
+    return tall ? base + 4 * e : base + (e >> 3) * row + 4 * (e & 7);
   }
-  // place of element j of group e in shared memory ([k][pitch])
-  __device__ __forceinline__ int place(int e, int j) const {
+  __device__ __forceinline__ void put4(int e, float4 v) const {
     if (tall) {
-      const int x = vec ? 4 * e + j : e, c = div(x);
-      return (x - c * k) * pitch + c;
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = div_k(4 * e + j);
+        u[(4 * e + j - c * k) * pitch + c] = x[j];
+      }
+    } else {
+      *reinterpret_cast<float4*>(u + (e >> 3) * pitch + 4 * (e & 7)) = v;
     }
-    const int r = div(e);
-    return r * pitch + (e - r * d) * (vec ? 4 : 1) + j;
+  }
+  __device__ __forceinline__ float4 get4(int e) const {
+    if (tall) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = div_k(4 * e + j);
+        x[j] = u[(4 * e + j - c * k) * pitch + c];
+      }
+      return make_float4(x[0], x[1], x[2], x[3]);
+    }
+    return *reinterpret_cast<const float4*>(u + (e >> 3) * pitch + 4 * (e & 7));
+  }
+  // element e < k * len <= 512, in memory's order
+  __device__ __forceinline__ int64_t offset(int e) const {
+    if (tall) return base + e;
+    const int r = e / len;
+    return base + r * row + (e - r * len);
+  }
+  __device__ __forceinline__ int place(int e) const {
+    const int c = tall ? div_k(e) : e / len;  // wide: the row
+    return tall ? (e - c * k) * pitch + c : c * pitch + e - c * len;
   }
 };
 
-constexpr int kBatch = 4;  // groups a thread loads at once
-
-template <int KB>
-__global__ void __launch_bounds__(kThreads) muon_kernel(const MuonArgs a) {
+// VEC: every matrix can be read four elements at a time (but for the columns
+// behind a multiple of 32).
+template <int KB, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) muon_kernel(const MuonArgs a) {
   constexpr int K = 8 * KB;
   constexpr int kBlocks = KB == 2 ? 3 : 1;  // 8 x 8 blocks of G's upper half
   extern __shared__ float u[];
@@ -129,125 +149,117 @@ __global__ void __launch_bounds__(kThreads) muon_kernel(const MuonArgs a) {
   const MuonSlot& sl = a.slot[id - layer * a.n_slots];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 
-  Tile t;
-  t.pitch = a.pitch;
-  t.tall = sl.rows > sl.cols;
-  t.k = min(sl.rows, sl.cols);
-  const int m = max(sl.rows, sl.cols);
-  t.row = sl.cols;
+  const bool tall = sl.rows > sl.cols;
+  const int k = min(sl.rows, sl.cols), m = max(sl.rows, sl.cols);
   const int64_t origin = layer * a.layer_stride + sl.off;
   const int tile = min(a.tile, ((m + C - 1) / C + 31) & ~31);
   const int n_tiles = (m + tile - 1) / tile;
   const bool resident = n_tiles <= C;
-  const bool base_ok = ((reinterpret_cast<uintptr_t>(a.w + origin) | reinterpret_cast<uintptr_t>(a.grad + origin) |
-                         reinterpret_cast<uintptr_t>(a.mom + origin)) & 15) == 0;
-  auto set_tile = [&](int i) {
-    const int j0 = i * tile;
-    t.len = min(tile, m - j0);
-    t.base = origin + static_cast<int64_t>(j0) * (t.tall ? t.k : 1);
-    t.vec = base_ok && ((t.tall ? t.k * t.len : sl.cols) & 3) == 0;
-    t.divisor(t.tall ? t.k : t.vec ? t.len >> 2 : t.len);
-  };
   const float mu = a.momentum;
   const bool nesterov = a.nesterov != 0;
-  // u of the tile into shared memory, zeros around it up to K rows and a
-  // multiple of 8 columns.  A thread's loads of kBatch groups are all issued
-  // before the first is used.
-  auto load_u = [&](bool first) {
-    const int l8 = (t.len + 7) & ~7;
-    const int n = t.groups();
-    if (t.vec) {
-      for (int e0 = threadIdx.x; e0 < n; e0 += kBatch * kThreads) {
-        float4 g[kBatch], b[kBatch];
+  // chunk at column c0 of tile i
+  auto chunk = [&](int i, int c0) {
+    Chunk q;
+    const int j0 = i * tile + c0;
+    q.base = origin + static_cast<int64_t>(j0) * (tall ? k : 1);
+    q.row = sl.cols;
+    q.u = u + c0;
+    q.pitch = a.pitch;
+    q.k = k;
+    q.len = min(kCols, min(m - j0, tile - c0));
+    q.tall = tall;
+    q.vec = VEC && q.len == kCols;
+    q.inv = k > 1 ? 0xffffffffu / static_cast<uint32_t>(k) + 1u : 0u;
+    return q;
+  };
+  auto columns = [&](int i) { return min(tile, m - i * tile); };
+  // u of the chunk into shared memory, zeros behind its columns.  A lane's
+  // loads are all issued before the first is used.
+  auto load_u = [&](const Chunk& q, bool first) {
+    if (q.vec) {
+      const int n = 8 * k;
+      float4 g[4], b[4];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int e = e0 + j * kThreads;
-          if (e < n) {
-            const int64_t o = t.offset(e);
-            g[j] = __ldg(reinterpret_cast<const float4*>(a.grad + o));
-            b[j] = *reinterpret_cast<const float4*>(a.mom + o);
-          }
+      for (int j = 0; j < 4; ++j) {
+        const int e = lane + 32 * j;
+        if (e < n) {
+          const int64_t o = q.offset4(e);
+          g[j] = __ldg(reinterpret_cast<const float4*>(a.grad + o));
+          b[j] = *reinterpret_cast<const float4*>(a.mom + o);
         }
+      }
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int e = e0 + j * kThreads;
-          if (e < n) {
-            float4 v = b[j];
-            if (first) {
-              v = make_float4(fmaf(mu, v.x, g[j].x), fmaf(mu, v.y, g[j].y), fmaf(mu, v.z, g[j].z),
-                              fmaf(mu, v.w, g[j].w));
-              *reinterpret_cast<float4*>(a.mom + t.offset(e)) = v;
-            }
-            if (nesterov)
-              v = make_float4(fmaf(mu, v.x, g[j].x), fmaf(mu, v.y, g[j].y), fmaf(mu, v.z, g[j].z),
-                              fmaf(mu, v.w, g[j].w));
-            if (t.tall) {
-              u[t.place(e, 0)] = v.x;
-              u[t.place(e, 1)] = v.y;
-              u[t.place(e, 2)] = v.z;
-              u[t.place(e, 3)] = v.w;
-            } else {
-              *reinterpret_cast<float4*>(u + t.place(e, 0)) = v;
-            }
+      for (int j = 0; j < 4; ++j) {
+        const int e = lane + 32 * j;
+        if (e < n) {
+          float4 v = b[j];
+          if (first) {
+            v = make_float4(fmaf(mu, v.x, g[j].x), fmaf(mu, v.y, g[j].y), fmaf(mu, v.z, g[j].z),
+                            fmaf(mu, v.w, g[j].w));
+            *reinterpret_cast<float4*>(a.mom + q.offset4(e)) = v;
           }
+          if (nesterov)
+            v = make_float4(fmaf(mu, v.x, g[j].x), fmaf(mu, v.y, g[j].y), fmaf(mu, v.z, g[j].z),
+                            fmaf(mu, v.w, g[j].w));
+          q.put4(e, v);
         }
       }
     } else {
-      for (int e0 = threadIdx.x; e0 < n; e0 += kBatch * kThreads) {
-        float g[kBatch], b[kBatch];
+      const int n = k * q.len;
+#pragma unroll 1
+      for (int e0 = lane; e0 < n; e0 += 32 * kScalar) {
+        float g[kScalar], b[kScalar];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int e = e0 + j * kThreads;
-          if (e < n) {
-            const int64_t o = t.offset(e);
+        for (int j = 0; j < kScalar; ++j) {
+          if (e0 + 32 * j < n) {
+            const int64_t o = q.offset(e0 + 32 * j);
             g[j] = __ldg(a.grad + o);
             b[j] = a.mom[o];
           }
         }
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int e = e0 + j * kThreads;
+        for (int j = 0; j < kScalar; ++j) {
+          const int e = e0 + 32 * j;
           if (e < n) {
             float v = b[j];
-            if (first) a.mom[t.offset(e)] = v = fmaf(mu, v, g[j]);
-            u[t.place(e, 0)] = nesterov ? fmaf(mu, v, g[j]) : v;
+            if (first) a.mom[q.offset(e)] = v = fmaf(mu, v, g[j]);
+            q.u[q.place(e)] = nesterov ? fmaf(mu, v, g[j]) : v;
           }
         }
       }
+      if (lane >= q.len)
+        for (int r = 0; r < k; ++r) q.u[r * q.pitch + lane] = 0.f;
     }
-    for (int e = threadIdx.x; e < (K - t.k) * l8; e += kThreads) {
-      const int r = e / l8;
-      u[(t.k + r) * t.pitch + e - r * l8] = 0.f;
-    }
-    for (int e = threadIdx.x; e < t.k * (l8 - t.len); e += kThreads) {
-      const int r = e / (l8 - t.len);
-      u[r * t.pitch + t.len + e - r * (l8 - t.len)] = 0.f;
-    }
+    __syncwarp();
   };
+  // rows k .. K - 1 stay zero: P's last rows and columns are a multiple of the identity's
+  for (int e = threadIdx.x; e < (K - k) * a.pitch; e += kThreads) u[k * a.pitch + e] = 0.f;
+  __syncthreads();
 
   // ------------------------------------------------------------ G = u u^T
   double acc[kBlocks][2];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) acc[b][0] = acc[b][1] = 0.0;
   for (int i = rank; i < n_tiles; i += C) {
-    set_tile(i);
-    __syncthreads();
-    load_u(true);
-    if (t.vec && resident) {  // w of the tile into L2 while the small matrices are worked on
-      for (int e = 8 * threadIdx.x; e < t.groups(); e += 8 * kThreads)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + t.offset(e)));
-    }
-    __syncthreads();
-    const float* p0 = u + (lane >> 2) * t.pitch + (lane & 3);
-    const float* p1 = p0 + 8 * t.pitch;
-#pragma unroll 4
-    for (int c = 4 * w; c < t.len; c += 4 * kWarps) {
-      const double x0 = static_cast<double>(p0[c]);
-      mma_f64(acc[0], x0, x0);
-      if constexpr (KB == 2) {
-        const double x1 = static_cast<double>(p1[c]);
-        mma_f64(acc[1], x0, x1);
-        mma_f64(acc[2], x1, x1);
+    const int cols = columns(i);
+    for (int c0 = kCols * w; c0 < cols; c0 += kCols * kWarps) {
+      const Chunk q = chunk(i, c0);
+      load_u(q, true);
+      if (resident && q.vec) {  // w of the chunk into L2 while the small matrices are worked on
+        for (int e = 8 * lane; e < 8 * k; e += 8 * 32)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + q.offset4(e)));
+      }
+      const float* p0 = q.u + (lane >> 2) * q.pitch + (lane & 3);
+      const float* p1 = p0 + 8 * q.pitch;
+#pragma unroll
+      for (int c = 0; c < kCols; c += 4) {
+        const double x0 = static_cast<double>(p0[c]);
+        mma_f64(acc[0], x0, x0);
+        if constexpr (KB == 2) {
+          const double x1 = static_cast<double>(p1[c]);
+          mma_f64(acc[1], x0, x1);
+          mma_f64(acc[2], x1, x1);
+        }
       }
     }
   }
@@ -298,7 +310,7 @@ __global__ void __launch_bounds__(kThreads) muon_kernel(const MuonArgs a) {
 
   // ------------------------------------------------- the steps, on K x K
   if (w == 0) {  // |u|_F^2 is G's trace
-    double d = lane < t.k ? G[lane * kLd + lane] : 0.0;
+    double d = lane < k ? G[lane * kLd + lane] : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (lane == 0) s_scale = 1.0 / (sqrt(d) + static_cast<double>(a.eps));
@@ -355,66 +367,89 @@ __global__ void __launch_bounds__(kThreads) muon_kernel(const MuonArgs a) {
                                    : sqrtf(fmaxf(1.f, static_cast<float>(sl.rows) / static_cast<float>(sl.cols)));
   const float step_size = a.lr * adjust, keep = 1.f - a.lr * a.weight_decay;
   for (int i = rank; i < n_tiles; i += C) {
-    if (!resident) {
-      set_tile(i);
-      __syncthreads();
-      load_u(false);
-      __syncthreads();
-    }
-    for (int c = 8 * w; c < t.len; c += 8 * kWarps) {
-      double x[2 * KB];
+    const int cols = columns(i);
+    for (int c0 = kCols * w; c0 < cols; c0 += kCols * kWarps) {
+      const Chunk q = chunk(i, c0);
+      if (!resident) load_u(q, false);
+      float4 v[4];  // w of the chunk, on its way while the products are formed
+      if (q.vec) {
 #pragma unroll
-      for (int s = 0; s < 2 * KB; ++s) x[s] = static_cast<double>(u[(4 * s + (lane & 3)) * t.pitch + c + (lane >> 2)]);
-      __syncwarp();  // the warp's 8 columns are read before they are overwritten
-#pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        double o[2] = {0.0, 0.0};
-#pragma unroll
-        for (int s = 0; s < 2 * KB; ++s) mma_f64(o, pf[b][s], x[s]);
-        *reinterpret_cast<float2*>(u + (8 * b + (lane >> 2)) * t.pitch + c + 2 * (lane & 3)) =
-            make_float2(static_cast<float>(o[0]), static_cast<float>(o[1]));
+        for (int j = 0; j < 4; ++j)
+          if (lane + 32 * j < 8 * k) v[j] = *reinterpret_cast<const float4*>(a.w + q.offset4(lane + 32 * j));
       }
-    }
-    __syncthreads();
-    const int n = t.groups();
-    if (t.vec) {
-      for (int e0 = threadIdx.x; e0 < n; e0 += kBatch * kThreads) {
-        float4 v[kBatch];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (e0 + j * kThreads < n) v[j] = *reinterpret_cast<const float4*>(a.w + t.offset(e0 + j * kThreads));
+      for (int c = 0; c < kCols; c += 8) {
+        double x[2 * KB];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int e = e0 + j * kThreads;
-          if (e < n) {
-            const float x0 = u[t.place(e, 0)], x1 = u[t.place(e, 1)], x2 = u[t.place(e, 2)], x3 = u[t.place(e, 3)];
-            *reinterpret_cast<float4*>(a.w + t.offset(e)) =
-                make_float4(fmaf(-step_size, x0, keep * v[j].x), fmaf(-step_size, x1, keep * v[j].y),
-                            fmaf(-step_size, x2, keep * v[j].z), fmaf(-step_size, x3, keep * v[j].w));
+        for (int s = 0; s < 2 * KB; ++s)
+          x[s] = static_cast<double>(q.u[(4 * s + (lane & 3)) * q.pitch + c + (lane >> 2)]);
+        __syncwarp();  // the 8 columns are read before they are overwritten
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          double o[2] = {0.0, 0.0};
+#pragma unroll
+          for (int s = 0; s < 2 * KB; ++s) mma_f64(o, pf[b][s], x[s]);
+          *reinterpret_cast<float2*>(q.u + (8 * b + (lane >> 2)) * q.pitch + c + 2 * (lane & 3)) =
+              make_float2(static_cast<float>(o[0]), static_cast<float>(o[1]));
+        }
+      }
+      __syncwarp();
+      if (q.vec) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = lane + 32 * j;
+          if (e < 8 * k) {
+            const float4 x = q.get4(e);
+            *reinterpret_cast<float4*>(a.w + q.offset4(e)) =
+                make_float4(fmaf(-step_size, x.x, keep * v[j].x), fmaf(-step_size, x.y, keep * v[j].y),
+                            fmaf(-step_size, x.z, keep * v[j].z), fmaf(-step_size, x.w, keep * v[j].w));
+          }
+        }
+      } else {
+        const int n = k * q.len;
+#pragma unroll 1
+        for (int e0 = lane; e0 < n; e0 += 32 * kScalar) {
+          float x[kScalar];
+#pragma unroll
+          for (int j = 0; j < kScalar; ++j)
+            if (e0 + 32 * j < n) x[j] = a.w[q.offset(e0 + 32 * j)];
+#pragma unroll
+          for (int j = 0; j < kScalar; ++j) {
+            const int e = e0 + 32 * j;
+            if (e < n) a.w[q.offset(e)] = fmaf(-step_size, q.u[q.place(e)], keep * x[j]);
           }
         }
       }
-    } else {
-      for (int e = threadIdx.x; e < n; e += kThreads) {
-        const int64_t o = t.offset(e);
-        a.w[o] = fmaf(-step_size, u[t.place(e, 0)], keep * a.w[o]);
-      }
+      __syncwarp();
     }
   }
   // whoever waits for this launch waits for the ones before it
   if (a.chained) pdl_wait();
 }
 
-template <int KB>
+template <int KB, bool VEC>
 cudaError_t launch(const MuonArgs& a, cudaStream_t st) {
   static std::atomic<unsigned long long> attr_set{0};
   cudaError_t e = once_per_device(attr_set, [] {
-    return cudaFuncSetAttribute(muon_kernel<KB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(muon_kernel<KB, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 8 * KB * (kMaxTile + 4) * static_cast<int>(sizeof(float)));
   });
   if (e != cudaSuccess) return e;
-  return launch_cluster(muon_kernel<KB>, static_cast<unsigned>(a.layers) * a.n_slots * a.cluster, kThreads, a.cluster,
-                        sizeof(float) * 8 * KB * a.pitch, st, a.chained, a);
+  return launch_cluster(muon_kernel<KB, VEC>, static_cast<unsigned>(a.layers) * a.n_slots * a.cluster, kThreads,
+                        a.cluster, sizeof(float) * 8 * KB * a.pitch, st, a.chained, a);
+}
+
+// Four elements at a time: 16-byte aligned bases and strides, and for the wide
+// layout rows of a multiple of four.
+bool vectors(const MuonArgs& a) {
+  uintptr_t bits = reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.grad) |
+                   reinterpret_cast<uintptr_t>(a.mom);
+  if (a.layers > 1) bits |= static_cast<uintptr_t>(a.layer_stride) * sizeof(float);
+  for (int i = 0; i < a.n_slots; ++i) {
+    bits |= static_cast<uintptr_t>(a.slot[i].off) * sizeof(float);
+    if (a.slot[i].rows <= a.slot[i].cols) bits |= static_cast<uintptr_t>(a.slot[i].cols) * sizeof(float);
+  }
+  return bits % 16 == 0;
 }
 
 }  // namespace
@@ -455,7 +490,9 @@ cudaError_t muon_update(MuonArgs all, cudaStream_t st) {
     a.pitch = a.tile + 4;
     if (static_cast<int64_t>(a.layers) * a.n_slots * C >= (1LL << 31)) return cudaErrorInvalidValue;
     a.chained = !first;
-    const cudaError_t e = k <= 8 ? launch<1>(a, st) : launch<2>(a, st);
+    const bool vec = vectors(a);
+    const cudaError_t e = k <= 8 ? (vec ? launch<1, true>(a, st) : launch<1, false>(a, st))
+                                 : (vec ? launch<2, true>(a, st) : launch<2, false>(a, st));
     if (e != cudaSuccess) return e;
     first = false;
   }
