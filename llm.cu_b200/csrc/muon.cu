@@ -24,12 +24,13 @@
 // small steps for itself.  Sides too long for the cluster's shared memory go
 // in several tiles a CTA, and the second pass forms u again from g and buf.
 //
-// 112 matrices of 16 x 2048 (73 MB) take 30 us, 11 at the copy rate.  The CTAs
-// of one wave go through their phases together: 6 us of loads at the copy
-// rate, then the 64-bit products (7 us of the tensor pipe, 16 cycles each), the
-// small steps (2 us of dependent products of about 55 cycles) and the
-// exchange of G's parts, then the stores.  All 224 of a 28-layer model's
-// attention adapters take 47 us, where AdamW's seven passes take 43.
+// 112 matrices of 16 x 2048 (73 MB) take 26 us, 11 at the copy rate: a CTA's
+// two passes take 7 us each, half of it the 64-bit products (7 us of an SM's
+// tensor pipe in all, 16 cycles each), the small steps 2 us of dependent
+// products (about 55 cycles each) and the exchange of G's parts 1 us.  Loading
+// a chunk ahead, or w into L2 beforehand, made neither pass faster.  All 224
+// matrices of a 28-layer model's attention adapters take 47 us, where AdamW's
+// seven passes take 43.
 #include <algorithm>
 #include <cmath>
 
@@ -245,10 +246,6 @@ __global__ void __launch_bounds__(kThreads, 2) muon_kernel(const MuonArgs a) {
     for (int c0 = kCols * w; c0 < cols; c0 += kCols * kWarps) {
       const Chunk q = chunk(i, c0);
       load_u(q, true);
-      if (resident && q.vec) {  // w of the chunk into L2 while the small matrices are worked on
-        for (int e = 8 * lane; e < 8 * k; e += 8 * 32)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + q.offset4(e)));
-      }
       const float* p0 = q.u + (lane >> 2) * q.pitch + (lane & 3);
       const float* p1 = p0 + 8 * q.pitch;
 #pragma unroll
@@ -461,7 +458,7 @@ cudaError_t muon_update(MuonArgs all, cudaStream_t st) {
     if (std::min(all.slot[i].rows, all.slot[i].cols) > kMuonMaxRank) return cudaErrorInvalidValue;
   // columns a CTA: 1024, less while that leaves SMs without one (every CTA of a
   // matrix runs the small steps, so wide tiles are cheaper: 112 matrices of 16 x
-  // 2048 take 30 us in pairs of CTAs and 35 in fours), down to 128
+  // 2048 take 26 us in pairs of CTAs and 32 in fours), down to 128
   int want = 1024;
   for (;; want /= 2) {
     int64_t ctas = 0;
