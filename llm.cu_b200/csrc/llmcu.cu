@@ -1618,9 +1618,9 @@ llmcu_status llmcu_preference_forward_backward(llmcu_ctx* ctx, const int32_t* to
     tl.pref.ref = ctx->tl_ref;
   }
   CKS(run_forward_backward(ctx, batch, seq, &tl));
-  if (rewards)
-    CK(cudaMemcpyAsync(rewards, ctx->tl_reward, sizeof(float) * batch, cudaMemcpyDeviceToHost, ctx->st));
-  return read_loss(ctx, loss_out);
+  CKS(read_loss(ctx, loss_out));  // the step has ended (within the deadline)
+  if (rewards) CK(cudaMemcpy(rewards, ctx->tl_reward, sizeof(float) * batch, cudaMemcpyDeviceToHost));
+  return LLMCU_OK;
 }
 
 llmcu_status llmcu_policy_forward_backward(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* targets,
@@ -1643,8 +1643,9 @@ llmcu_status llmcu_policy_forward_backward(llmcu_ctx* ctx, const int32_t* tokens
     tl.policy.ref = ctx->tl_ref;
   }
   CKS(run_forward_backward(ctx, batch, seq, &tl));
-  if (stats) CK(cudaMemcpyAsync(stats, ctx->tl_stats, 4 * sizeof(float), cudaMemcpyDeviceToHost, ctx->st));
-  return read_loss(ctx, loss_out);
+  CKS(read_loss(ctx, loss_out));
+  if (stats) CK(cudaMemcpy(stats, ctx->tl_stats, 4 * sizeof(float), cudaMemcpyDeviceToHost));
+  return LLMCU_OK;
 }
 
 llmcu_status llmcu_muon(llmcu_ctx* ctx, const llmcu_muon_cfg* cfg) {

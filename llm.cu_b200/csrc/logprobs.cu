@@ -73,7 +73,7 @@ template <int MR>
 __global__ void __launch_bounds__(kFewThreads, kFewBlocks)
     few_rows_kernel(const __half* __restrict__ x, const __half* __restrict__ E, const int* __restrict__ targets, int M,
                     int H, int V, int ldx, int lde, float2* __restrict__ part, float* __restrict__ tgt_logit) {
-  extern __shared__ float xs[];  // [MR][h256]
+  extern __shared__ __align__(16) float xs[];  // [MR][h256]
   __shared__ float2 red[kFewThreads / 32][MR];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int h256 = (H + 255) & ~255;
@@ -351,8 +351,10 @@ __global__ void __launch_bounds__(256)
   __syncthreads();
   pdl_wait();
   const int at = place ? place[m] : m;  // the row of the partial sums; -1: it has no gradient
+  const float up = dlogp[m];
+  const bool live = ok && at >= 0 && up != 0.f;  // else 0, whatever x and the sums hold
   // 1 - p_t without cancellation for a confident token
-  const float g = ok ? scale * dlogp[m] : 0.f;
+  const float g = scale * up;
   const float one_minus = ok ? -expm1f(s_exact - lse[m]) : 0.f;
   const float unshift = exp2f(-kProbShift);
   const __half* et = E + static_cast<size_t>(ok ? t : 0) * lde;
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(256)
   const bool vec = (reinterpret_cast<uintptr_t>(dx) & 7) == 0 && (lddx & 3) == 0;
   for (int c = threadIdx.x * 4; c < H; c += blockDim.x * 4) {
     float r[4] = {0.f, 0.f, 0.f, 0.f};
-    if (ok && at >= 0) {
+    if (live) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = 0; k < slabs; ++k) {  // ld_acc is a multiple of 4; what lies past H is not used
         const float4 o = *reinterpret_cast<const float4*>(a0 + static_cast<size_t>(k) * slab_rows * ld_acc + c);

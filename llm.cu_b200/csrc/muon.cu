@@ -136,7 +136,7 @@ template <int KB, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) muon_kernel(const MuonArgs a) {
   constexpr int K = 8 * KB;
   constexpr int kBlocks = KB == 2 ? 3 : 1;  // 8 x 8 blocks of G's upper half
-  extern __shared__ float u[];
+  extern __shared__ __align__(16) float u[];
   __shared__ double gw[kWarps / 2][kBlocks * 64];
   __shared__ double slots[8][kBlocks * 64];  // G's parts, every CTA's
   __shared__ double G[K * kLd], Q[K * kLd], T[K * kLd], P[2][K * kLd];
@@ -258,6 +258,7 @@ __global__ void __launch_bounds__(kThreads, 2) muon_kernel(const MuonArgs a) {
           mma_f64(acc[2], x1, x1);
         }
       }
+      __syncwarp();  // a later tile's chunk lands in the same place
     }
   }
   // the warps' parts: the upper half's first, then the lower half's on top

@@ -158,6 +158,8 @@ def test_lm_logprobs_backward_rows_without_gradient(llmcu, cuda_device, M, live)
     d2 = torch.where(off & half, float("nan"), d2)
     got = lm_backward(llmcu, x, E, t2, lse, d2, 16.0)
     assert (got[off] == 0).all()
+    x[off], lse[off] = float("nan"), float("nan")
+    assert torch.equal(lm_backward(llmcu, x, E, t2, lse, d2, 16.0), got)
     # rows land in other tiles: the tensor cores' sums over K do not depend on the row
     assert torch.equal(got[on], full[on])
     assert llmcu.kernel_checks(stream()) == 0
