@@ -888,14 +888,15 @@ struct EpiLogProb {
 #pragma unroll
       for (int j = 0; j < 32; ++j) mq = fmaxf(mq, v[j]);
       if (mq > -INFINITY) {
-        const float r2 = mq * kLog2e;
+        // the difference first: a rounded mq * log2(e) would scale every term by
+        // up to 1 + |mq| 2^-24, which a confident token's log-probability shows
         float a = 0.f, b = 0.f;
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-          a += fast_exp2(fmaf(v[j], kLog2e, -r2));
-          b += fast_exp2(fmaf(v[j + 1], kLog2e, -r2));
+          a += fast_exp2((v[j] - mq) * kLog2e);
+          b += fast_exp2((v[j + 1] - mq) * kLog2e);
         }
-        s = fmaf(s, fast_exp2(fmaf(m, kLog2e, -r2)), a + b);
+        s = fmaf(s, fast_exp2((m - mq) * kLog2e), a + b);
         m = mq;
       } else {  // -inf so far, or NaN among -inf: the sum keeps the NaN
 #pragma unroll

@@ -236,9 +236,9 @@ __global__ void __launch_bounds__(kRows* kWarps)
       const float rough = tgt_logit[row], d = exact - rough;
       if (isfinite(d)) s = fmaf(exp2f((rough - p.x) * kLog2e), expm1f(d), s);
     }
-    const float l = p.x + logf(s);
-    lse[row] = l;
-    logp[row] = ok ? exact - l : 0.f;
+    const float ls = logf(s);
+    lse[row] = p.x + ls;
+    logp[row] = ok ? (exact - p.x) - ls : 0.f;  // not through lse, whose rounding a confident token would show
   }
 }
 
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps)
   if (lane == 0) {
     const float rough = tgt_logit[m], d = exact - rough;
     if (isfinite(d)) s = fmaf(exp2f((rough - mx) * kLog2e), expm1f(d), s);
-    logp[m] = exact - (mx + logf(s));
+    logp[m] = (exact - mx) - logf(s);
   }
 }
 

@@ -189,10 +189,11 @@ def test_lm_logprobs_gradient_by_differences(llmcu, cuda_device):
     within(fp - fm, slope, tol)
 
 
-def test_lm_logprobs_banned_and_extreme_logits(llmcu, cuda_device):
+@pytest.mark.parametrize("M", [1, 2, 6])
+def test_lm_logprobs_banned_and_extreme_logits(llmcu, cuda_device, M):
     """Rows of E that push their logits to -inf (banned ids) take no probability;
     logits of +-20000 neither overflow nor underflow the whole."""
-    M, H, V = 6, 64, 600
+    H, V = 64, 600
     x = torch.ones(M, H, device=cuda_device, dtype=torch.float16)
     E = (torch.randn(V, H, device=cuda_device, generator=torch.Generator(device=cuda_device).manual_seed(0)) * 0.1).half()
     E[::3] = float("-inf")
@@ -204,9 +205,18 @@ def test_lm_logprobs_banned_and_extreme_logits(llmcu, cuda_device):
     within(logp, torch.log_softmax(z, 1)[:, 1], 1e-4)
     E = torch.zeros(V, H, device=cuda_device, dtype=torch.float16)
     E[5], E[300] = 312.5, -312.5  # logits of +-20000
-    logp, lse = lm_forward(llmcu, x, E, torch.tensor([5, 300, 0, 5, 300, 0], device=cuda_device, dtype=torch.int32))
+    logp, lse = lm_forward(llmcu, x, E, torch.tensor([5, 300, 0, 5, 300, 0], device=cuda_device, dtype=torch.int32)[:M])
     assert lse.tolist() == [20000.0] * M
-    assert logp.tolist() == [0.0, -40000.0, -20000.0] * 2
+    assert logp.tolist() == ([0.0, -40000.0, -20000.0] * 2)[:M]
+    # a row whose every logit is -inf, and one with a NaN: no probability, no wrong number
+    E[:] = float("-inf")
+    logp, lse = lm_forward(llmcu, x, E, torch.zeros(M, device=cuda_device, dtype=torch.int32))
+    assert (lse == float("-inf")).all() and logp.isnan().all()
+    E.zero_()
+    x[0, 3] = float("nan")
+    logp, lse = lm_forward(llmcu, x, E, torch.zeros(M, device=cuda_device, dtype=torch.int32))
+    assert lse[0].isnan() and logp[0].isnan()
+    assert torch.allclose(lse[1:], torch.full_like(lse[1:], math.log(V)), rtol=1e-6)
 
 
 # ------------------------------------------------------------- preference loss
