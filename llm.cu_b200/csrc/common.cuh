@@ -343,8 +343,9 @@ struct PolicyArgs {
   float* dlogp;                   // [batch, ld]; nullable
   int batch, seq, ld;
   int agg, token_adv;
-  float beta, inv_norm;                // inv_norm: kPolicyConstant
-  float low, high, dual;               // the clip's bounds on r (dual: on r for A < 0)
+  float beta;
+  double inv_norm;                     // kPolicyConstant
+  float low, high, dual;               // the clip's bounds on r, less 1 (dual: for A < 0)
   double log_low, log_high, log_dual;  // their logarithms; -inf / inf where there is none
   // set by policy_loss
   float f_low, f_high, f_dual;  // the logarithms in fp32

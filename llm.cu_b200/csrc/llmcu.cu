@@ -1094,13 +1094,12 @@ bool policy_args(const llmcu_policy_cfg* cfg, PolicyArgs* a) {
   a->agg = cfg->agg;
   a->token_adv = cfg->token_advantages;
   a->beta = cfg->kl_beta;
-  a->inv_norm = cfg->agg == LLMCU_POLICY_CONSTANT ? static_cast<float>(1.0 / cfg->norm) : 0.f;
-  const double low = 1.0 - cfg->clip_low, high = 1.0 + cfg->clip_high;
-  a->low = static_cast<float>(low);
-  a->high = static_cast<float>(high);
-  a->dual = cfg->dual_clip;
+  a->inv_norm = cfg->agg == LLMCU_POLICY_CONSTANT ? 1.0 / cfg->norm : 0.0;
+  a->low = -cfg->clip_low;
+  a->high = cfg->clip_high;
+  a->dual = static_cast<float>(static_cast<double>(cfg->dual_clip) - 1.0);
   // a ratio is never below 1 - clip_low where that is 0 or less
-  a->log_low = low > 0.0 ? std::log1p(-static_cast<double>(cfg->clip_low)) : -INFINITY;
+  a->log_low = cfg->clip_low < 1.f ? std::log1p(-static_cast<double>(cfg->clip_low)) : -INFINITY;
   a->log_high = std::log1p(static_cast<double>(cfg->clip_high));
   a->log_dual = cfg->dual_clip > 0.f ? std::log(static_cast<double>(cfg->dual_clip)) : INFINITY;
   return true;

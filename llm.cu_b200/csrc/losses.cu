@@ -269,17 +269,47 @@ __global__ void __launch_bounds__(kThreads)
 // border; next to it (which fp32 cannot tell) in 64 bits, so that the token
 // falls on the side that the inputs say.
 //
-// e^d - d - 1 loses everything to cancellation for a small d; below 1 its
-// series d^2 (1/2! + d/3! + ...) is summed instead, to d^12 / 12! (the next
-// term is under 2^-25 of the sum), and e^d - 1 is d more.
+// Advantages are centred as a rule, so the sum of r A over a batch is a small
+// difference of large terms: with e = r - 1 it is taken as the sum of A, in 64
+// bits, and the sum of e A, whose terms are several times smaller.
+//
+// e^x - 1 and e^d - d - 1 lose everything to cancellation for a small argument;
+// below 1 the series x^2 (1/2! + x/3! + ...) is summed, to x^12 / 12! (the next
+// term is under 2^-25 of the sum).
+// Returns e^x - x - 1; *em1 = e^x - 1, *ex = e^x.
+__device__ __forceinline__ float exp_rest(float x, float* em1, float* ex) {
+  float s = 1.f / 479001600.f;
+  s = fmaf(s, x, 1.f / 39916800.f);
+  s = fmaf(s, x, 1.f / 3628800.f);
+  s = fmaf(s, x, 1.f / 362880.f);
+  s = fmaf(s, x, 1.f / 40320.f);
+  s = fmaf(s, x, 1.f / 5040.f);
+  s = fmaf(s, x, 1.f / 720.f);
+  s = fmaf(s, x, 1.f / 120.f);
+  s = fmaf(s, x, 1.f / 24.f);
+  s = fmaf(s, x, 1.f / 6.f);
+  s = fmaf(s, x, 0.5f);
+  float rest = x * x * s;
+  *em1 = x + rest;
+  *ex = 1.f + *em1;
+  if (!(fabsf(x) < 1.f)) {
+    *ex = expf(x);
+    *em1 = *ex - 1.f;
+    rest = *em1 - x;
+  }
+  return rest;
+}
+
 struct PolicyToken {
-  float loss, kl, grad;
+  float loss;  // the loss less -A
+  float kl, grad;
   bool clip;
 };
 __device__ __forceinline__ PolicyToken policy_token(const PolicyArgs& a, float lp, float old, float A, float ref) {
   PolicyToken t;
   const float delta = lp - old;
-  const float rA = expf(delta) * A;
+  float e, r;
+  exp_rest(delta, &e, &r);
   // clips above hi and below lo
   const bool pos = A > 0.f;
   const float hi = pos ? a.f_high : a.f_dual, lo = pos ? -INFINITY : a.f_low;
@@ -290,29 +320,13 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyArgs& a, float l
     below = !pos && d64 < a.log_low;
   }
   t.clip = (above || below) && (pos || A < 0.f);
-  const float bound = below ? a.low : pos ? a.high : a.dual;
-  t.loss = t.clip ? -bound * A : -rA;
-  t.grad = t.clip ? 0.f : -rA;
+  const float bound = below ? a.low : pos ? a.high : a.dual;  // less 1, as e
+  t.loss = t.clip ? -bound * A : -e * A;
+  t.grad = t.clip ? 0.f : -r * A;
   t.kl = 0.f;
   if (a.ref) {
-    const float d = ref - lp;
-    float s = 1.f / 479001600.f;
-    s = fmaf(s, d, 1.f / 39916800.f);
-    s = fmaf(s, d, 1.f / 3628800.f);
-    s = fmaf(s, d, 1.f / 362880.f);
-    s = fmaf(s, d, 1.f / 40320.f);
-    s = fmaf(s, d, 1.f / 5040.f);
-    s = fmaf(s, d, 1.f / 720.f);
-    s = fmaf(s, d, 1.f / 120.f);
-    s = fmaf(s, d, 1.f / 24.f);
-    s = fmaf(s, d, 1.f / 6.f);
-    s = fmaf(s, d, 0.5f);
-    t.kl = d * d * s;
-    float em1 = d + t.kl;
-    if (!(fabsf(d) < 1.f)) {
-      em1 = expf(d) - 1.f;
-      t.kl = em1 - d;
-    }
+    float em1, unused;
+    t.kl = exp_rest(ref - lp, &em1, &unused);
     t.grad = fmaf(-a.beta, em1, t.grad);
     t.loss = fmaf(a.beta, t.kl, t.loss);
   }
@@ -386,17 +400,23 @@ struct PolicyQuad {
     v[2] = x.z;
     v[3] = x.w;
   }
-  __device__ __forceinline__ void run(const PolicyArgs& a, uint32_t bits, float weight, float (&g)[4], float& loss,
-                                      float& kl, int& clips) const {
+  // gradients times `weight`; the quad's loss, KL terms and clipped tokens added up
+  __device__ __forceinline__ void run(const PolicyArgs& a, uint32_t bits, float weight, float (&g)[4], double& loss,
+                                      double& kl, int& clips) const {
+    float l = 0.f, n = 0.f;
+    double adv_sum = 0.0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const PolicyToken t = policy_token(a, lp[j], old[j], adv[j], ref[j]);
       const bool on = (bits >> j) & 1;
       g[j] = on ? t.grad * weight : 0.f;
-      loss += on ? t.loss : 0.f;
-      kl += on ? t.kl : 0.f;
+      l += on ? t.loss : 0.f;
+      n += on ? t.kl : 0.f;
       clips += on && t.clip;
+      adv_sum += static_cast<double>(on ? adv[j] : 0.f);
     }
+    loss += static_cast<double>(l) - adv_sum;
+    kl += static_cast<double>(n);
   }
 };
 
@@ -435,12 +455,12 @@ __global__ void __launch_bounds__(kSmallThreads) policy_small_kernel(PolicyArgs 
   PolicyQuad quad;
   if (bits) quad.load(a, p);
   if (by_row && bits) atomicAdd(&rows[p.row], __popc(bits));
-  float weight = a.inv_norm;
+  double weight = a.inv_norm;
   if (a.agg == kPolicyTokenMean) {
     double n[1] = {static_cast<double>(__popc(bits))};
     block_sums(n, red);
     cluster_sums(n, slots[0], C, rank, true);
-    weight = static_cast<float>(1.0 / fmax(n[0], 1.0));
+    weight = 1.0 / fmax(n[0], 1.0);
   } else if (by_row) {
     if (C > 1) cluster_wait();
     __syncthreads();
@@ -453,15 +473,15 @@ __global__ void __launch_bounds__(kSmallThreads) policy_small_kernel(PolicyArgs 
     if (bits) {
       int n = 0;
       for (int c = 0; c < C; ++c) n += all_rows[c * a.batch + p.row];
-      weight = 1.0f / (static_cast<float>(n) * static_cast<float>(a.batch));
+      weight = 1.0 / (static_cast<double>(n) * static_cast<double>(a.batch));
     }
   }
-  float g[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, kl = 0.f;
+  float g[4] = {0.f, 0.f, 0.f, 0.f};
+  double l = 0.0, kl = 0.0;
   int clips = 0;
-  if (bits) quad.run(a, bits, weight, g, l, kl, clips);
+  if (bits) quad.run(a, bits, static_cast<float>(weight), g, l, kl, clips);
   if (a.dlogp) p.store(a, g);
-  double v[4] = {static_cast<double>(l * weight), static_cast<double>(kl), static_cast<double>(clips),
-                 static_cast<double>(__popc(bits))};
+  double v[4] = {l * weight, kl, static_cast<double>(clips), static_cast<double>(__popc(bits))};
   block_sums(v, red);
   cluster_sums(v, slots[1], C, rank, a.agg == kPolicyConstant, false);
   if (rank == 0 && threadIdx.x == 0) write_stats(v, a.stats);
@@ -482,9 +502,11 @@ __device__ __forceinline__ int count16(const PolicyArgs& a, int64_t i, int64_t f
   return n;
 }
 
-// Scored tokens: of each row (one CTA or warp a row) into counts[row], or of
-// everything, a partial sum a CTA, into counts[0 .. gridDim.x).
-__global__ void __launch_bounds__(kThreads) policy_count_kernel(PolicyArgs a, int* __restrict__ counts) {
+// Means over rows: the rows' weights, 1 / (batch * scored tokens), into
+// weights[row] (one CTA or warp a row); else the scored tokens of everything, a
+// partial sum a CTA, into counts[0 .. gridDim.x).
+__global__ void __launch_bounds__(kThreads)
+    policy_count_kernel(PolicyArgs a, int* __restrict__ counts, double* __restrict__ weights) {
   pdl_trigger();
   __shared__ int red[kThreads / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -497,7 +519,7 @@ __global__ void __launch_bounds__(kThreads) policy_count_kernel(PolicyArgs a, in
     const int row = blockIdx.x * (kThreads / 32) + w;
     if (row < a.batch) count_row(row, lane, 32);
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0 && row < a.batch) counts[row] = n;
+    if (lane == 0 && row < a.batch) weights[row] = 1.0 / (static_cast<double>(max(n, 1)) * static_cast<double>(a.batch));
     return;
   }
   if (a.agg == kPolicySequenceMean) {  // a CTA a row
@@ -519,22 +541,31 @@ __global__ void __launch_bounds__(kThreads) policy_count_kernel(PolicyArgs a, in
   __syncthreads();
   if (w == 0) {
     n = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? red[lane] : 0);
-    if (lane == 0) counts[blockIdx.x] = n;
+    if (lane == 0) {
+      if (a.agg == kPolicySequenceMean)
+        weights[blockIdx.x] = 1.0 / (static_cast<double>(max(n, 1)) * static_cast<double>(a.batch));
+      else
+        counts[blockIdx.x] = n;
+    }
   }
 }
 
 __global__ void __launch_bounds__(kThreads, kMainBlocks)
-    policy_main_kernel(PolicyArgs a, const int* __restrict__ counts, int n_counts, double* __restrict__ partial) {
+    policy_main_kernel(PolicyArgs a, const int* __restrict__ counts, int n_counts, const double* __restrict__ weights,
+                       double* __restrict__ partial) {
   pdl_trigger();
   pdl_wait();
   __shared__ double red[4 * 32];
-  float weight = a.inv_norm;
+  double weight = a.inv_norm;  // of every token, but for means over rows: of the sums
   if (a.agg == kPolicyTokenMean) {
     double n[1] = {0.0};
     for (int i = threadIdx.x; i < n_counts; i += kThreads) n[0] += static_cast<double>(counts[i]);
     block_sums(n, red);
-    weight = static_cast<float>(1.0 / fmax(n[0], 1.0));
+    weight = 1.0 / fmax(n[0], 1.0);
   }
+  const bool by_row = a.agg == kPolicySequenceMean;
+  if (by_row) weight = 1.0;
+  float each = static_cast<float>(weight);
   double v[4] = {0.0, 0.0, 0.0, 0.0};
   int clips = 0;
   int64_t tokens = 0;
@@ -556,16 +587,20 @@ __global__ void __launch_bounds__(kThreads, kMainBlocks)
       next_bits = next.mask(a);
     }
     if (bits) {
-      if (a.agg == kPolicySequenceMean)
-        weight = 1.0f / (static_cast<float>(counts[p.row]) * static_cast<float>(a.batch));
-      float l = 0.f, kl = 0.f;
-      quad.run(a, bits, weight, g, l, kl, clips);
-      v[0] += static_cast<double>(l * weight);
-      v[1] += static_cast<double>(kl);
+      if (by_row) {
+        const double w = weights[p.row];
+        each = static_cast<float>(w);
+        double l = 0.0;
+        quad.run(a, bits, each, g, l, v[1], clips);
+        v[0] += l * w;
+      } else {
+        quad.run(a, bits, each, g, v[0], v[1], clips);
+      }
       tokens += __popc(bits);
     }
     if (a.dlogp) p.store(a, g);
   }
+  v[0] *= weight;
   v[2] = static_cast<double>(clips);
   v[3] = static_cast<double>(tokens);
   block_sums(v, red);
@@ -613,7 +648,7 @@ cudaError_t preference_loss(PreferenceArgs a, cudaStream_t st) {
 
 size_t policy_loss_workspace(int batch) {
   const size_t partial = sizeof(double) * 4 * kMainBlocks * static_cast<size_t>(gemm_num_sms());
-  return partial + sizeof(int) * std::max<size_t>(kCountBlocks, static_cast<size_t>(batch));
+  return partial + std::max(sizeof(int) * kCountBlocks, sizeof(double) * static_cast<size_t>(batch));
 }
 
 cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
@@ -649,6 +684,7 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
   }
   double* partial = static_cast<double*>(ws);
   int* counts = reinterpret_cast<int*>(partial + 4 * kMainBlocks * static_cast<size_t>(gemm_num_sms()));
+  double* weights = reinterpret_cast<double*>(counts);  // the one or the other
   const bool was = pdl_enabled();
   set_pdl(false);
   cudaError_t e = cudaSuccess;
@@ -659,11 +695,11 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
     n_counts = static_cast<int>(std::min<int64_t>(kCountBlocks, (a.units / 4 + kThreads - 1) / kThreads + 1));
   }
   if (n_counts) {
-    e = launch_pdl(policy_count_kernel, n_counts, kThreads, 0, st, a, counts);
+    e = launch_pdl(policy_count_kernel, n_counts, kThreads, 0, st, a, counts, weights);
     set_pdl(true);
   }
   const int blocks = policy_blocks(a.units);
-  if (e == cudaSuccess) e = launch_pdl(policy_main_kernel, blocks, kThreads, 0, st, a, counts, n_counts, partial);
+  if (e == cudaSuccess) e = launch_pdl(policy_main_kernel, blocks, kThreads, 0, st, a, counts, n_counts, weights, partial);
   set_pdl(true);
   if (e == cudaSuccess) e = launch_pdl(policy_stats_kernel, 1, kThreads, 0, st, partial, blocks, a.stats);
   set_pdl(was);
