@@ -276,28 +276,50 @@ __global__ void __launch_bounds__(kThreads)
 // e^x - 1 and e^d - d - 1 lose everything to cancellation for a small argument;
 // below 1 the series x^2 (1/2! + x/3! + ...) is summed, to x^12 / 12! (the next
 // term is under 2^-25 of the sum).
-// Returns e^x - x - 1; *em1 = e^x - 1, *ex = e^x.
-__device__ __forceinline__ float exp_rest(float x, float* em1, float* ex) {
-  float s = 1.f / 479001600.f;
-  s = fmaf(s, x, 1.f / 39916800.f);
-  s = fmaf(s, x, 1.f / 3628800.f);
-  s = fmaf(s, x, 1.f / 362880.f);
-  s = fmaf(s, x, 1.f / 40320.f);
-  s = fmaf(s, x, 1.f / 5040.f);
-  s = fmaf(s, x, 1.f / 720.f);
-  s = fmaf(s, x, 1.f / 120.f);
-  s = fmaf(s, x, 1.f / 24.f);
-  s = fmaf(s, x, 1.f / 6.f);
-  s = fmaf(s, x, 0.5f);
-  float rest = x * x * s;
-  *em1 = x + rest;
-  *ex = 1.f + *em1;
-  if (!(fabsf(x) < 1.f)) {
-    *ex = expf(x);
-    *em1 = *ex - 1.f;
-    rest = *em1 - x;
+//
+// Two tokens go through the series together (fma.rn.f32x2): the kernel is short
+// of issue slots.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float (&f)[2]) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f[0]), "=f"(f[1]) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+// rest = e^x - x - 1, em1 = e^x - 1, ex = e^x of two numbers.
+__device__ __forceinline__ void exp_rest2(const float (&x)[2], float (&rest)[2], float (&em1)[2], float (&ex)[2]) {
+  const uint64_t X = pack2(x[0], x[1]);
+  auto both = [](float c) { return pack2(c, c); };
+  uint64_t S = both(1.f / 479001600.f);
+  S = fma2(S, X, both(1.f / 39916800.f));
+  S = fma2(S, X, both(1.f / 3628800.f));
+  S = fma2(S, X, both(1.f / 362880.f));
+  S = fma2(S, X, both(1.f / 40320.f));
+  S = fma2(S, X, both(1.f / 5040.f));
+  S = fma2(S, X, both(1.f / 720.f));
+  S = fma2(S, X, both(1.f / 120.f));
+  S = fma2(S, X, both(1.f / 24.f));
+  S = fma2(S, X, both(1.f / 6.f));
+  S = fma2(S, X, both(0.5f));
+  float s[2];
+  unpack2(S, s);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    rest[j] = x[j] * x[j] * s[j];
+    em1[j] = x[j] + rest[j];
+    ex[j] = 1.f + em1[j];
+    if (!(fabsf(x[j]) < 1.f)) {
+      ex[j] = expf(x[j]);
+      em1[j] = ex[j] - 1.f;
+      rest[j] = em1[j] - x[j];
+    }
   }
-  return rest;
 }
 
 struct PolicyToken {
@@ -305,32 +327,40 @@ struct PolicyToken {
   float kl, grad;
   bool clip;
 };
-__device__ __forceinline__ PolicyToken policy_token(const PolicyArgs& a, float lp, float old, float A, float ref) {
-  PolicyToken t;
-  const float delta = lp - old;
-  float e, r;
-  exp_rest(delta, &e, &r);
-  // clips above hi and below lo
-  const bool pos = A > 0.f;
-  const float hi = pos ? a.f_high : a.f_dual, lo = pos ? -INFINITY : a.f_low;
-  bool above = delta > hi, below = delta < lo;
-  if (fminf(fabsf(delta - hi), fabsf(delta - lo)) < a.near) {
-    const double d64 = static_cast<double>(lp) - static_cast<double>(old);
-    above = d64 > (pos ? a.log_high : a.log_dual);
-    below = !pos && d64 < a.log_low;
+__device__ __forceinline__ void policy_tokens(const PolicyArgs& a, const float (&lp)[2], const float (&old)[2],
+                                              const float (&adv)[2], const float (&ref)[2], PolicyToken (&t)[2]) {
+  const float delta[2] = {lp[0] - old[0], lp[1] - old[1]};
+  float rest[2], e[2], r[2];
+  exp_rest2(delta, rest, e, r);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float A = adv[j];
+    // clips above hi and below lo
+    const bool pos = A > 0.f;
+    const float hi = pos ? a.f_high : a.f_dual, lo = pos ? -INFINITY : a.f_low;
+    bool above = delta[j] > hi, below = delta[j] < lo;
+    if (fminf(fabsf(delta[j] - hi), fabsf(delta[j] - lo)) < a.near) {
+      const double d64 = static_cast<double>(lp[j]) - static_cast<double>(old[j]);
+      above = d64 > (pos ? a.log_high : a.log_dual);
+      below = !pos && d64 < a.log_low;
+    }
+    t[j].clip = (above || below) && (pos || A < 0.f);
+    const float bound = below ? a.low : pos ? a.high : a.dual;  // less 1, as e
+    t[j].loss = t[j].clip ? -bound * A : -e[j] * A;
+    t[j].grad = t[j].clip ? 0.f : -r[j] * A;
+    t[j].kl = 0.f;
   }
-  t.clip = (above || below) && (pos || A < 0.f);
-  const float bound = below ? a.low : pos ? a.high : a.dual;  // less 1, as e
-  t.loss = t.clip ? -bound * A : -e * A;
-  t.grad = t.clip ? 0.f : -r * A;
-  t.kl = 0.f;
   if (a.ref) {
-    float em1, unused;
-    t.kl = exp_rest(ref - lp, &em1, &unused);
-    t.grad = fmaf(-a.beta, em1, t.grad);
-    t.loss = fmaf(a.beta, t.kl, t.loss);
+    const float d[2] = {ref[0] - lp[0], ref[1] - lp[1]};
+    float kl[2], em1[2], unused[2];
+    exp_rest2(d, kl, em1, unused);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      t[j].kl = kl[j];
+      t[j].grad = fmaf(-a.beta, em1[j], t[j].grad);
+      t[j].loss = fmaf(a.beta, kl[j], t[j].loss);
+    }
   }
-  return t;
 }
 
 // Unit u: four places of a row, of which the row's tokens are set in `in`
@@ -406,14 +436,20 @@ struct PolicyQuad {
     float l = 0.f, n = 0.f;
     double adv_sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const PolicyToken t = policy_token(a, lp[j], old[j], adv[j], ref[j]);
-      const bool on = (bits >> j) & 1;
-      g[j] = on ? t.grad * weight : 0.f;
-      l += on ? t.loss : 0.f;
-      n += on ? t.kl : 0.f;
-      clips += on && t.clip;
-      adv_sum += static_cast<double>(on ? adv[j] : 0.f);
+    for (int h = 0; h < 4; h += 2) {
+      const float x[2] = {lp[h], lp[h + 1]}, o[2] = {old[h], old[h + 1]}, A[2] = {adv[h], adv[h + 1]},
+                  rf[2] = {ref[h], ref[h + 1]};
+      PolicyToken t[2];
+      policy_tokens(a, x, o, A, rf, t);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const bool on = (bits >> (h + j)) & 1;
+        g[h + j] = on ? t[j].grad * weight : 0.f;
+        l += on ? t[j].loss : 0.f;
+        n += on ? t[j].kl : 0.f;
+        clips += on && t[j].clip;
+        adv_sum += static_cast<double>(on ? A[j] : 0.f);
+      }
     }
     loss += static_cast<double>(l) - adv_sum;
     kl += static_cast<double>(n);
