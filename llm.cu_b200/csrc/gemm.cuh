@@ -94,6 +94,7 @@ struct GemmSmem {
 struct EpiCtx {
   int lane;
   int row0;                 // first tile row of this warp (global row index)
+  int in_row0;              // the same before a K split's row offset: the row of A it belongs to
   int row;                  // this thread's row = row0 + lane
   int M, N;
   uint32_t slab;            // shared address of the 4 KB staging slab
@@ -433,7 +434,7 @@ struct EpiStoreF32 {
   static constexpr bool kStores = true;
   __device__ static void begin(State&, const Params&, const EpiCtx&, int) {}
   __device__ static bool chunk(State&, const Params& p, EpiCtx& c, int col0, const float* v) {
-    if (col0 >= c.N) return true;
+    if (col0 >= c.N || c.in_row0 >= c.M) return true;  // none of these rows exists
     slab_wait_read(c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -865,7 +866,7 @@ struct EpiLogProb {
   static constexpr bool kTmemDirect = true;
   __device__ static void begin(State&, const Params&, const EpiCtx&, int) {}
   __device__ static bool tile(State&, const Params& p, EpiCtx& c, int col0, uint32_t taddr, int) {
-    if (col0 >= c.N) return true;
+    if (col0 >= c.N || c.row0 >= c.M) return true;  // no row of this warp's 32 exists
     const int nv = min(128, c.N - col0);
     const bool live = c.row < c.M;
     const int t = live ? __ldg(p.targets + c.row) - col0 : -1;
@@ -931,7 +932,7 @@ struct EpiProbs {
   static constexpr bool kTmemDirect = true;
   __device__ static void begin(State&, const Params&, const EpiCtx&, int) {}
   __device__ static bool tile(State&, const Params& p, EpiCtx& c, int col0, uint32_t taddr, int) {
-    if (col0 >= c.N) return true;
+    if (col0 >= c.N || c.row0 >= c.M) return true;  // no row of this warp's 32 exists
     const int nv = min(128, c.N - col0);
     const bool live = c.row < c.M;
     const int t = live ? __ldg(p.targets + c.row) - (p.vocab_off + col0) : -1;
@@ -1338,7 +1339,8 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
       const int tm = sh.n_fastest ? tile / sh.tiles_n : tile % tiles_m;
       const int tn = sh.n_fastest ? tile % sh.tiles_n : tile / tiles_m;
       // split s -> its row block of partials; the odd CTA of a pair owns rows 128..255
-      c.row0 = (sp * sh.split_row_tiles + tm) * kRowsPerTile + static_cast<int>(rank) * kBlockM + ew * 32;
+      c.in_row0 = tm * kRowsPerTile + static_cast<int>(rank) * kBlockM + ew * 32;
+      c.row0 = sp * sh.split_row_tiles * kRowsPerTile + c.in_row0;
       c.row = c.row0 + lane;
       const uint32_t tbase = tmem_base + lane_off + acc * BN;
       typename Epi::State st;

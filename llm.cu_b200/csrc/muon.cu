@@ -76,7 +76,7 @@ __device__ __forceinline__ void small_product(const double* A, const double* B, 
 // step: loading, G, the product with P and the update of w, without a word to
 // the other warps, so that the warps' loads and products overlap.
 constexpr int kCols = 32;
-constexpr int kScalar = 4;  // single elements a lane loads at once
+constexpr int kScalar = 8;  // single elements a lane loads at once
 struct Chunk {
   int64_t base;  // its first element in the buffers
   int64_t row;   // wide: elements between rows
@@ -118,15 +118,21 @@ struct Chunk {
     }
     return *reinterpret_cast<const float4*>(u + (e >> 3) * pitch + 4 * (e & 7));
   }
-  // element e < k * len <= 512, in memory's order
-  __device__ __forceinline__ int64_t offset(int e) const {
-    if (tall) return base + e;
-    const int r = e / len;
-    return base + r * row + (e - r * len);
+  // Single elements, kScalar of them at a time for each lane: turn h < turns().
+  // Wide: rows kScalar h, ..., the lane's column.  Tall: in memory's order.
+  __device__ __forceinline__ int turns() const {
+    return tall ? (k * len + 32 * kScalar - 1) / (32 * kScalar) : (k + kScalar - 1) / kScalar;
   }
-  __device__ __forceinline__ int place(int e) const {
-    const int c = tall ? div_k(e) : e / len;  // wide: the row
-    return tall ? (e - c * k) * pitch + c : c * pitch + e - c * len;
+  __device__ __forceinline__ bool has(int h, int j, int lane) const {
+    return tall ? (h * kScalar + j) * 32 + lane < k * len : h * kScalar + j < k && lane < len;
+  }
+  __device__ __forceinline__ int64_t offset(int h, int j, int lane) const {
+    return tall ? base + (h * kScalar + j) * 32 + lane : base + (h * kScalar + j) * row + lane;
+  }
+  __device__ __forceinline__ int place(int h, int j, int lane) const {
+    if (!tall) return (h * kScalar + j) * pitch + lane;
+    const int e = (h * kScalar + j) * 32 + lane, c = div_k(e);
+    return (e - c * k) * pitch + c;
   }
 };
 
@@ -206,25 +212,23 @@ __global__ void __launch_bounds__(kThreads, 2) muon_kernel(const MuonArgs a) {
         }
       }
     } else {
-      const int n = k * q.len;
 #pragma unroll 1
-      for (int e0 = lane; e0 < n; e0 += 32 * kScalar) {
+      for (int h = 0; h < q.turns(); ++h) {
         float g[kScalar], b[kScalar];
 #pragma unroll
         for (int j = 0; j < kScalar; ++j) {
-          if (e0 + 32 * j < n) {
-            const int64_t o = q.offset(e0 + 32 * j);
+          if (q.has(h, j, lane)) {
+            const int64_t o = q.offset(h, j, lane);
             g[j] = __ldg(a.grad + o);
             b[j] = a.mom[o];
           }
         }
 #pragma unroll
         for (int j = 0; j < kScalar; ++j) {
-          const int e = e0 + 32 * j;
-          if (e < n) {
+          if (q.has(h, j, lane)) {
             float v = b[j];
-            if (first) a.mom[q.offset(e)] = v = fmaf(mu, v, g[j]);
-            q.u[q.place(e)] = nesterov ? fmaf(mu, v, g[j]) : v;
+            if (first) a.mom[q.offset(h, j, lane)] = v = fmaf(mu, v, g[j]);
+            q.u[q.place(h, j, lane)] = nesterov ? fmaf(mu, v, g[j]) : v;
           }
         }
       }
@@ -404,18 +408,16 @@ __global__ void __launch_bounds__(kThreads, 2) muon_kernel(const MuonArgs a) {
           }
         }
       } else {
-        const int n = k * q.len;
 #pragma unroll 1
-        for (int e0 = lane; e0 < n; e0 += 32 * kScalar) {
+        for (int h = 0; h < q.turns(); ++h) {
           float x[kScalar];
 #pragma unroll
           for (int j = 0; j < kScalar; ++j)
-            if (e0 + 32 * j < n) x[j] = a.w[q.offset(e0 + 32 * j)];
+            if (q.has(h, j, lane)) x[j] = a.w[q.offset(h, j, lane)];
 #pragma unroll
-          for (int j = 0; j < kScalar; ++j) {
-            const int e = e0 + 32 * j;
-            if (e < n) a.w[q.offset(e)] = fmaf(-step_size, q.u[q.place(e)], keep * x[j]);
-          }
+          for (int j = 0; j < kScalar; ++j)
+            if (q.has(h, j, lane))
+              a.w[q.offset(h, j, lane)] = fmaf(-step_size, q.u[q.place(h, j, lane)], keep * x[j]);
         }
       }
       __syncwarp();
