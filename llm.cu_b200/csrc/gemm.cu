@@ -203,16 +203,16 @@ cudaError_t dispatch(Epi epi, const EpiArgs& ea, const CUtensorMap* maps, const 
         return cudaErrorInvalidValue;
       }
     case Epi::kLogProb:
-      if constexpr (BN == 256 && !BMN) {
-        return launch<BN, EpiLogProb, BMN, CG>(maps, sh, EpiLogProb::Params{ea.targets, ea.part2, ea.tgt_logit}, err,
-                                               st);
+      if constexpr (BN >= 128 && !BMN) {
+        using E = EpiLogProb<BN / 128>;
+        return launch<BN, E, BMN, CG>(maps, sh, typename E::Params{ea.targets, ea.part2, ea.tgt_logit}, err, st);
       } else {
         return cudaErrorInvalidValue;
       }
     case Epi::kProbs:
-      if constexpr (BN == 256 && !BMN) {
-        return launch<BN, EpiProbs, BMN, CG>(maps, sh, EpiProbs::Params{ea.targets, ea.lse, ea.vocab_off},
-                                             err, st);
+      if constexpr (BN >= 128 && !BMN) {
+        using E = EpiProbs<BN / 128>;
+        return launch<BN, E, BMN, CG>(maps, sh, typename E::Params{ea.targets, ea.lse, ea.vocab_off}, err, st);
       } else {
         return cudaErrorInvalidValue;
       }
@@ -289,8 +289,8 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
   if (epi == Epi::kCEStream && (!ea.targets || !ea.ce_ref || !ea.part_max || !ea.part_sum || !ea.tgt_logit ||
                                 ea.vocab_off % 128 || ea.ce_slots < (ea.vocab_off + N + 127) / 128))
     return cudaErrorInvalidValue;
-  if (epi == Epi::kLogProb && (BN != 256 || !ea.targets || !ea.part2 || !ea.tgt_logit)) return cudaErrorInvalidValue;
-  if (epi == Epi::kProbs && (BN != 256 || !ea.targets || !ea.lse)) return cudaErrorInvalidValue;
+  if (epi == Epi::kLogProb && ((BN != 256 && BN != 128) || !ea.targets || !ea.part2 || !ea.tgt_logit)) return cudaErrorInvalidValue;
+  if (epi == Epi::kProbs && ((BN != 256 && BN != 128) || !ea.targets || !ea.lse)) return cudaErrorInvalidValue;
   if (ea.ksplit > 1 && (epi != Epi::kStoreF32 || (!ea.accumulate && !ea.slab_rows))) return cudaErrorInvalidValue;
   if (ea.slab_rows && (ea.slab_rows % (2 * kBlockM) || ea.slab_rows < M)) return cudaErrorInvalidValue;
   const int n_main = ea.n_main > 0 ? ea.n_main : N;
@@ -364,6 +364,7 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
   sh.fx_cnt = nullptr;
   sh.b_scale = B.mn ? nullptr : B.q8_scale;
   sh.m_rows = ea.m_rows;
+  sh.k_rotate = epi == Epi::kLogProb || epi == Epi::kProbs;
   if (ea.ksplit > 1) {  // K slices reduce-add into the same rows
     const int nk = sh.kb_per_split;
     const int kbps = (nk + ea.ksplit - 1) / ea.ksplit;

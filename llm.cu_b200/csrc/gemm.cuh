@@ -64,6 +64,11 @@ struct GemmShape {
   // rows really there (at most M; null: M), counted on the device by an
   // earlier kernel: row tiles past them are not run, and M only bounds them
   const int* m_rows;
+  // 1: column tile tn starts its K loop at block tn % (K blocks) and goes round,
+  // so that CTAs in step do not read the same columns of B's rows at once --
+  // with rows a power of two apart these lie in few memory channels.  The
+  // order of the sum over K then depends on the tile, not on the run.
+  int k_rotate;
 };
 
 constexpr int kBlockM = 128;
@@ -852,7 +857,11 @@ struct EpiCEStream {
 // the target's logit; the logits themselves go nowhere.  The pairs lie
 // [slot][row], so a warp's 32 rows store 256 contiguous bytes.  A row whose
 // slot is all -inf leaves (-inf, 0).
+// G: epilogue warps per TMEM lane quadrant, each with a slot of 128 columns
+// (two for 256-wide tiles, one for 128-wide ones).
+template <int G>
 struct EpiLogProb {
+  static constexpr int kEpiGroups = G;
   struct Params {
     const int* targets;  // [M]
     float2* part;        // [slots, M]
@@ -918,7 +927,9 @@ struct EpiLogProb {
 // tensor cores' product with E needs; the target's column, whose p - 1 it
 // would spoil for a confident token, is stored as 0 and added in fp32 by the
 // finishing kernel.
+template <int G>
 struct EpiProbs {
+  static constexpr int kEpiGroups = G;
   struct Params {
     const int* targets;  // [M]
     const float* lse;    // [M]
@@ -1070,7 +1081,7 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
   const int nk = (sh.K + kBlockK - 1) / kBlockK;
   int tiles_m = sh.tiles_m, num_tiles = sh.num_tiles;
   int num_units = num_tiles * sh.splits;  // (tile, K split) work units
-  if (warp == 0 && lane == 0 && unit0 < num_units && !sh.m_rows) {
+  if (warp == 0 && lane == 0 && unit0 < num_units && !sh.m_rows && !sh.k_rotate) {
     // while the previous kernel finishes: the first unit's first stages of A
     // and B into L2.  A prefetch only fills L2, which stays coherent with that
     // kernel's writes; the loads into shared memory wait for it below.
@@ -1112,7 +1123,9 @@ __global__ void __launch_bounds__(64 + 32 * EW + (Q8 ? kQ8Threads : 0), 1)
         const int kb_end = min(nk, (sp + 1) * sh.kb_per_split);
         const int arow = tm * kRowsPerTile + static_cast<int>(rank) * kBlockM;
         const int brow = tn * BN + static_cast<int>(rank) * kBRows;
-        for (int kb = sp * sh.kb_per_split; kb < kb_end; ++kb, ++it) {
+        const int rot = sh.k_rotate ? tn % nk : 0;
+        for (int kb0 = sp * sh.kb_per_split; kb0 < kb_end; ++kb0, ++it) {
+          const int kb = kb0 + rot < nk ? kb0 + rot : kb0 + rot - nk;
           const int s = it % STAGES;
           const uint32_t par = ((it / STAGES) & 1) ^ 1;
           if (!mbar_wait(&empty[s], par, abort_flag, err, kErrWaitConsumer)) { ok = false; break; }

@@ -49,59 +49,42 @@ __device__ __forceinline__ float target_logit(const __half* __restrict__ x, cons
   return warp_sum(s);
 }
 
-constexpr int kRows = 32;   // rows per CTA of the forward's finishing kernel: one per lane
-constexpr int kWarps = 32;  // its warps share the slots
+constexpr int kWarps = 32;  // of the forward's finishing kernel: they share the slots
 
-// Few rows (M <= kFewRows): the vocabulary is read once by plain loads and
-// multiplied on the CUDA cores, in fp32.  What bounds it is reading E: 622 MB
-// for 151936 x 2048 is 95 us at the measured copy rate.  The GEMM, whose tiles
-// of 256 columns take five rounds for 4.01 rounds' worth of work there, runs
-// 133 to 138 us; this kernel 106 us for one row and 116 for two.  With four
-// rows (148 us) the products outweigh the loads.
+// One row: the vocabulary is read once by plain loads and multiplied on the
+// CUDA cores, in fp32.  What bounds it is reading E: 622 MB for 151936 x 2048
+// is 95 us at the measured copy rate; with its finishing kernel it takes 103.
+// The GEMM takes 110 us there for one row as for sixteen, this kernel 113 for
+// two and 148 for four: the products would outweigh the loads.
 //
 // A warp takes four rows of E at a time, a lane eight elements of each every
 // 256; x lies in shared memory as fp32, its halves of eight apart, so that a
-// warp's 16-byte reads meet every bank once.  The four logits of each x row
-// meet in all lanes, which keep its running maximum and sum.
-constexpr int kFewRows = 2;
-constexpr int kFewThreads = 512;
-constexpr int kFewBlocks = 2;  // CTAs an SM
-constexpr int kFewSmem = 96 * 1024;
+// warp's 16-byte reads meet every bank once.  The four logits meet in all
+// lanes, which keep the running maximum and sum.
+constexpr int kOneThreads = 512;
+constexpr int kOneBlocks = 2;  // CTAs an SM
+constexpr int kOneSmem = 96 * 1024;
 constexpr int kVecRows = 4;    // rows of E a warp takes at once
 
-template <int MR>
-__global__ void __launch_bounds__(kFewThreads, kFewBlocks)
-    few_rows_kernel(const __half* __restrict__ x, const __half* __restrict__ E, const int* __restrict__ targets, int M,
-                    int H, int V, int ldx, int lde, float2* __restrict__ part, float* __restrict__ tgt_logit) {
-  extern __shared__ __align__(16) float xs[];  // [MR][h256]
-  __shared__ float2 red[kFewThreads / 32][MR];
+__global__ void __launch_bounds__(kOneThreads, kOneBlocks)
+    one_row_kernel(const __half* __restrict__ x, const __half* __restrict__ E, const int* __restrict__ targets, int H,
+                   int V, int lde, float2* __restrict__ part, float* __restrict__ tgt_logit) {
+  extern __shared__ __align__(16) float xs[];  // [h256]
+  __shared__ float2 red[kOneThreads / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int h256 = (H + 255) & ~255;
-  for (int e = threadIdx.x; e < MR * h256; e += kFewThreads) {
-    const int m = e / h256, k = e - m * h256;
-    const float v = m < M && k < H ? __half2float(x[static_cast<size_t>(m) * ldx + k]) : 0.f;
-    xs[m * h256 + (k & ~255) + (k & 4) * 32 + ((k & 255) >> 3) * 4 + (k & 3)] = v;
-  }
+  for (int k = threadIdx.x; k < h256; k += kOneThreads)
+    xs[(k & ~255) + (k & 4) * 32 + ((k & 255) >> 3) * 4 + (k & 3)] = k < H ? __half2float(x[k]) : 0.f;
   pdl_trigger();
   __syncthreads();
-  float mx[MR], sum[MR];
-  int t[MR];
-#pragma unroll
-  for (int m = 0; m < MR; ++m) {
-    mx[m] = -INFINITY;
-    sum[m] = 0.f;
-    t[m] = m < M ? targets[m] : -1;
-  }
+  float2 p = make_float2(-INFINITY, 0.f);
+  const int t = *targets;
   // a run of E's rows for each warp of the grid
-  const int warps = gridDim.x * (kFewThreads / 32);
-  const int me = blockIdx.x * (kFewThreads / 32) + w;
+  const int warps = gridDim.x * (kOneThreads / 32);
+  const int me = blockIdx.x * (kOneThreads / 32) + w;
   const int v_end = static_cast<int>(static_cast<int64_t>(V) * (me + 1) / warps);
   for (int v0 = static_cast<int>(static_cast<int64_t>(V) * me / warps); v0 < v_end; v0 += kVecRows) {
-    float acc[kVecRows][MR];
-#pragma unroll
-    for (int r = 0; r < kVecRows; ++r)
-#pragma unroll
-      for (int m = 0; m < MR; ++m) acc[r][m] = 0.f;
+    float acc[kVecRows] = {};
     const __half* row[kVecRows];  // past the run: its last row again, not used
 #pragma unroll
     for (int r = 0; r < kVecRows; ++r) row[r] = E + static_cast<size_t>(min(v0 + r, v_end - 1)) * lde;
@@ -121,112 +104,98 @@ __global__ void __launch_bounds__(kFewThreads, kFewBlocks)
             if (k + j < H) h[j] = row[r][k + j];
         }
       }
-      float f[kVecRows][8];
+      const float4 a = *reinterpret_cast<const float4*>(xs + k0 + lane * 4);
+      const float4 b = *reinterpret_cast<const float4*>(xs + k0 + 128 + lane * 4);
 #pragma unroll
       for (int r = 0; r < kVecRows; ++r) {
         const __half2* h = reinterpret_cast<const __half2*>(&e[r]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 v = __half22float2(h[j]);
-          f[r][2 * j] = v.x;
-          f[r][2 * j + 1] = v.y;
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MR; ++m) {
-        const float4 a = *reinterpret_cast<const float4*>(xs + m * h256 + k0 + lane * 4);
-        const float4 b = *reinterpret_cast<const float4*>(xs + m * h256 + k0 + 128 + lane * 4);
-#pragma unroll
-        for (int r = 0; r < kVecRows; ++r) {
-          float c = acc[r][m];
-          c = fmaf(a.x, f[r][0], c);
-          c = fmaf(a.y, f[r][1], c);
-          c = fmaf(a.z, f[r][2], c);
-          c = fmaf(a.w, f[r][3], c);
-          c = fmaf(b.x, f[r][4], c);
-          c = fmaf(b.y, f[r][5], c);
-          c = fmaf(b.z, f[r][6], c);
-          acc[r][m] = fmaf(b.w, f[r][7], c);
-        }
+        const float2 f0 = __half22float2(h[0]), f1 = __half22float2(h[1]), f2 = __half22float2(h[2]),
+                     f3 = __half22float2(h[3]);
+        float c = acc[r];
+        c = fmaf(a.x, f0.x, c);
+        c = fmaf(a.y, f0.y, c);
+        c = fmaf(a.z, f1.x, c);
+        c = fmaf(a.w, f1.y, c);
+        c = fmaf(b.x, f2.x, c);
+        c = fmaf(b.y, f2.y, c);
+        c = fmaf(b.z, f3.x, c);
+        acc[r] = fmaf(b.w, f3.y, c);
       }
     }
+    float l[kVecRows];
+    float n = p.x;
 #pragma unroll
-    for (int m = 0; m < MR; ++m) {
-      float l[kVecRows];
-      float n = mx[m];
+    for (int r = 0; r < kVecRows; ++r) {
+      const float v = warp_sum(acc[r]);
+      l[r] = v0 + r < v_end ? v : -INFINITY;
+      if (v0 + r == t && v0 + r < v_end && lane == 0) *tgt_logit = v;
+      n = fmaxf(n, l[r]);
+    }
+    if (n > -INFINITY) {
+      float s = p.y * exp2f((p.x - n) * kLog2e);
 #pragma unroll
-      for (int r = 0; r < kVecRows; ++r) {
-        const float v = warp_sum(acc[r][m]);
-        l[r] = v0 + r < v_end ? v : -INFINITY;
-        if (v0 + r == t[m] && v0 + r < v_end && lane == 0) tgt_logit[m] = v;
-        n = fmaxf(n, l[r]);
-      }
-      if (n > -INFINITY) {
-        float s = sum[m] * exp2f((mx[m] - n) * kLog2e);
+      for (int r = 0; r < kVecRows; ++r) s += exp2f((l[r] - n) * kLog2e);
+      p = make_float2(n, s);
+    } else {  // -inf so far, or NaN: the sum keeps the NaN
 #pragma unroll
-        for (int r = 0; r < kVecRows; ++r) s += exp2f((l[r] - n) * kLog2e);
-        sum[m] = s;
-        mx[m] = n;
-      } else {  // -inf so far, or NaN: the sum keeps the NaN
-#pragma unroll
-        for (int r = 0; r < kVecRows; ++r) sum[m] += l[r] == -INFINITY ? 0.f : l[r];
-      }
+      for (int r = 0; r < kVecRows; ++r) p.y += l[r] == -INFINITY ? 0.f : l[r];
     }
   }
-  if (lane == 0) {
-#pragma unroll
-    for (int m = 0; m < MR; ++m) red[w][m] = make_float2(mx[m], sum[m]);
-  }
+  if (lane == 0) red[w] = p;
   __syncthreads();
-  if (threadIdx.x < MR && threadIdx.x < M) {
-    float2 a = red[0][threadIdx.x];
-    for (int i = 1; i < kFewThreads / 32; ++i) a = join_pairs(a, red[i][threadIdx.x]);
-    part[static_cast<size_t>(blockIdx.x) * M + threadIdx.x] = a;
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kOneThreads / 32; ++i) p = join_pairs(p, red[i]);
+    part[blockIdx.x] = p;
   }
 }
 
-template <int MR>
-cudaError_t few_rows(const __half* x, const __half* E, const int* targets, int M, int H, int V, int ldx, int lde,
-                     float2* part, float* tgt_logit, int blocks, cudaStream_t st) {
+cudaError_t one_row(const __half* x, const __half* E, const int* targets, int H, int V, int lde, float2* part,
+                    float* tgt_logit, int blocks, cudaStream_t st) {
   static std::atomic<unsigned long long> attr_set{0};
   cudaError_t e = once_per_device(attr_set, [] {
-    return cudaFuncSetAttribute(few_rows_kernel<MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+    return cudaFuncSetAttribute(one_row_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOneSmem);
   });
   if (e != cudaSuccess) return e;
-  const size_t smem = sizeof(float) * MR * ((H + 255) & ~255);
-  return launch_pdl(few_rows_kernel<MR>, blocks, kFewThreads, smem, st, x, E, targets, M, H, V, ldx, lde, part,
-                    tgt_logit);
+  return launch_pdl(one_row_kernel, blocks, kOneThreads, sizeof(float) * ((H + 255) & ~255), st, x, E, targets, H, V,
+                    lde, part, tgt_logit);
 }
 
-// Joins the slots' (max, sum) pairs of 32 rows: warp w takes slots w, w + 32,
-// ...; lanes are rows, so every load is 256 contiguous bytes.  Before that,
-// while the GEMM still runs, warp w forms row w's target logit (x, E and the
-// targets are complete before the GEMM starts); it also replaces the GEMM's
-// value in the sum.
-__global__ void __launch_bounds__(kRows* kWarps)
+// Joins the slots' (max, sum) pairs, RB rows a CTA: lane l of warp w takes row
+// l % RB of slots w * (32 / RB) + l / RB, and every 32 * (32 / RB)th on.  Before
+// that, while the GEMM still runs, warp w forms row w's target logit (x, E and
+// the targets are complete before the GEMM starts); it also replaces the GEMM's
+// value in the sum.  Four rows a CTA (32-byte pieces of the pairs, [slot][row])
+// while that is at most two CTAs an SM, else 32; at most 32 warps a CTA, fewer
+// where there are fewer slots to share.
+template <int RB>
+__global__ void __launch_bounds__(32 * kWarps)
     logprob_finish_kernel(const float2* __restrict__ part, const float* __restrict__ tgt_logit,
                           const int* __restrict__ targets, const __half* __restrict__ x, const __half* __restrict__ E,
                           int M, int H, int V, int ldx, int lde, int slots, float* __restrict__ logp,
                           float* __restrict__ lse) {
   pdl_trigger();
-  __shared__ float2 red[kWarps][kRows + 1];  // + 1: read down its columns
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int row = blockIdx.x * kRows + w;
-  const int t = row < M ? targets[row] : -1;
+  __shared__ float2 red[kWarps][RB + 1];  // + 1: read down its columns
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  const int row = blockIdx.x * RB + w;
+  const int t = w < RB && row < M ? targets[row] : -1;
   const bool ok = t >= 0 && t < V;
   float exact = 0.f;
   if (ok) exact = target_logit(x + static_cast<size_t>(row) * ldx, E + static_cast<size_t>(t) * lde, H, lane);
   pdl_wait();
-  const int m = blockIdx.x * kRows + lane;
+  const int m = blockIdx.x * RB + lane % RB;
   float2 p = make_float2(-INFINITY, 0.f);
   if (m < M) {
 #pragma unroll 4
-    for (int i = w; i < slots; i += kWarps) p = join_pairs(p, part[static_cast<size_t>(i) * M + m]);
+    for (int i = w * (32 / RB) + lane / RB; i < slots; i += nw * (32 / RB))
+      p = join_pairs(p, part[static_cast<size_t>(i) * M + m]);
   }
-  red[w][lane] = p;
+#pragma unroll
+  for (int o = 16; o >= RB; o >>= 1)
+    p = join_pairs(p, make_float2(__shfl_xor_sync(0xffffffffu, p.x, o), __shfl_xor_sync(0xffffffffu, p.y, o)));
+  if (lane < RB) red[w][lane] = p;
   __syncthreads();
-  if (row >= M) return;
-  p = red[lane][w];  // the 32 parts of row w
+  if (w >= RB || row >= M) return;
+  p = lane < nw ? red[lane][w] : make_float2(-INFINITY, 0.f);  // the warps' parts of row w
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     p = join_pairs(p, make_float2(__shfl_xor_sync(0xffffffffu, p.x, o), __shfl_xor_sync(0xffffffffu, p.y, o)));
@@ -286,22 +255,29 @@ __global__ void __launch_bounds__(1024)
   __shared__ int warps[32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int base = 0;
-  for (int m0 = 0; m0 < M; m0 += 1024) {
-    const int m = m0 + threadIdx.x;
-    const bool live = m < M && targets[m] >= 0 && targets[m] < V && dlogp[m] != 0.f;
-    const uint32_t b = __ballot_sync(0xffffffffu, live);
-    if (lane == 0) warps[w] = __popc(b);
-    __syncthreads();
-    int before = 0, total = 0;
-    for (int i = 0; i < 32; ++i) {
-      before += i < w ? warps[i] : 0;
-      total += warps[i];
+  for (int m0 = 0; m0 < M; m0 += 4 * 1024) {
+    bool live[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // the loads of four turns at once
+      const int m = m0 + j * 1024 + threadIdx.x;
+      live[j] = m < M && targets[m] >= 0 && targets[m] < V && dlogp[m] != 0.f;
     }
-    const int at = base + before + __popc(b & ((1u << lane) - 1u));
-    if (live) list[at] = m;
-    if (m < M) place[m] = live ? at : -1;
-    base += total;
-    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = m0 + j * 1024 + threadIdx.x;
+      if (m0 + j * 1024 >= M) break;
+      const uint32_t b = __ballot_sync(0xffffffffu, live[j]);
+      if (lane == 0) warps[w] = __popc(b);
+      __syncthreads();
+      const int mine = warps[lane];
+      const int total = __reduce_add_sync(0xffffffffu, mine);
+      const int before = __reduce_add_sync(0xffffffffu, lane < w ? mine : 0);
+      const int at = base + before + __popc(b & ((1u << lane) - 1u));
+      if (live[j]) list[at] = m;
+      if (m < M) place[m] = live[j] ? at : -1;
+      base += total;
+      __syncthreads();
+    }
   }
   if (threadIdx.x == 0) *count = base;
 }
@@ -332,41 +308,45 @@ __global__ void __launch_bounds__(256)
 }
 
 // dx row m from the K slices' partial sums (slab k: rows [k * slab_rows, ...)
-// of acc), in slice order, and the target's own term in fp32.
+// of acc), in slice order, and the target's own term in fp32.  A warp takes
+// `cols` columns of a row (parts of them for each row).
 __global__ void __launch_bounds__(256)
     logprob_dx_kernel(const float* __restrict__ acc, int slabs, int slab_rows, int ld_acc,
-                      const int* __restrict__ place,
-                      const __half* __restrict__ x, int ldx, const __half* __restrict__ E, int lde,
-                      const float* __restrict__ lse, const float* __restrict__ dlogp, const int* __restrict__ targets,
-                      int H, int V, float scale, __half* __restrict__ dx, int lddx) {
+                      const int* __restrict__ place, const __half* __restrict__ x, int ldx,
+                      const __half* __restrict__ E, int lde, const float* __restrict__ lse,
+                      const float* __restrict__ dlogp, const int* __restrict__ targets, int M, int H, int V,
+                      float scale, __half* __restrict__ dx, int lddx, int cols, int parts) {
   pdl_trigger();
-  __shared__ float s_exact;
-  const int m = blockIdx.x;
+  const int lane = threadIdx.x & 31;
+  const int64_t item = blockIdx.x * static_cast<int64_t>(8) + (threadIdx.x >> 5);
+  const int m = static_cast<int>(item / parts);
+  if (m >= M) return;
+  const int c0 = static_cast<int>(item - static_cast<int64_t>(m) * parts) * cols;
   const int t = targets[m];
   const bool ok = t >= 0 && t < V;
-  if (ok && threadIdx.x < 32) {  // inputs alone: while the last GEMM still runs
-    const float l = target_logit(x + static_cast<size_t>(m) * ldx, E + static_cast<size_t>(t) * lde, H, threadIdx.x);
-    if (threadIdx.x == 0) s_exact = l;
-  }
-  __syncthreads();
+  const __half* et = E + static_cast<size_t>(ok ? t : 0) * lde;
+  // inputs alone: while the last GEMM still runs
+  const float exact = ok ? target_logit(x + static_cast<size_t>(m) * ldx, et, H, lane) : 0.f;
+  const float up = dlogp[m];
+  // 1 - p_t without cancellation for a confident token
+  const float one_minus = ok ? -expm1f(exact - lse[m]) : 0.f;
   pdl_wait();
   const int at = place ? place[m] : m;  // the row of the partial sums; -1: it has no gradient
-  const float up = dlogp[m];
   const bool live = ok && at >= 0 && up != 0.f;  // else 0, whatever x and the sums hold
-  // 1 - p_t without cancellation for a confident token
   const float g = scale * up;
-  const float one_minus = ok ? -expm1f(s_exact - lse[m]) : 0.f;
   const float unshift = exp2f(-kProbShift);
-  const __half* et = E + static_cast<size_t>(ok ? t : 0) * lde;
   const float* a0 = acc + static_cast<size_t>(max(at, 0)) * ld_acc;
+  const size_t slab = static_cast<size_t>(slab_rows) * ld_acc;
   __half* out = dx + static_cast<size_t>(m) * lddx;
   const bool vec = (reinterpret_cast<uintptr_t>(dx) & 7) == 0 && (lddx & 3) == 0;
-  for (int c = threadIdx.x * 4; c < H; c += blockDim.x * 4) {
+  const int end = min(H, c0 + cols);
+  for (int c = c0 + lane * 4; c < end; c += 128) {
     float r[4] = {0.f, 0.f, 0.f, 0.f};
     if (live) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
       for (int k = 0; k < slabs; ++k) {  // ld_acc is a multiple of 4; what lies past H is not used
-        const float4 o = *reinterpret_cast<const float4*>(a0 + static_cast<size_t>(k) * slab_rows * ld_acc + c);
+        const float4 o = *reinterpret_cast<const float4*>(a0 + k * slab + c);
         v.x += o.x;
         v.y += o.y;
         v.z += o.z;
@@ -431,10 +411,20 @@ BwdPlan bwd_plan(int M, int H, int V) {
   return p;
 }
 
-// More rows than one CTA pair's tile: the ones without a gradient (prompts,
-// padding, clipped tokens) are left out of both products.  The copy of the
-// others costs about 10 us of 4.5 ms at 4096 x 2048 x 151936.
-constexpr int kGatherRows = 256;
+// The rows without a gradient (prompts, padding, clipped tokens) are left out
+// of both products where these cost more than the two kernels and the copy that
+// it takes, about 10 us: from 2^33 products on (26 us at the tensor cores' full
+// rate), and with more rows than one CTA pair's tile.
+bool gathers(int M, int H, int V) {
+  return M > 256 && static_cast<double>(M) * H * V >= static_cast<double>(1LL << 33);
+}
+
+// Tile width of the products with the vocabulary: 256 columns, but up to 128
+// rows (one CTA a tile) 128 while these take one round: 77 rows of 872 x 3032
+// then take 12.3 us, else 16.  (With more rounds the wider tiles read E faster:
+// 16 rows of 2048 x 151936 take 121 us in five rounds of 256 columns, 141 in
+// nine of 128.)
+int tile_width(int M, int N) { return M <= 128 && (N + 127) / 128 <= gemm_num_sms() ? 128 : 256; }
 
 // rows for the TMA and for 16-byte loads
 bool rows_ok(const __half* p, int ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
@@ -451,7 +441,7 @@ struct PdlScope {  // the chain's kernels await one another (pdl_wait); the firs
 size_t lm_logprobs_workspace(int M, int H, int V, bool backward) {
   if (!backward) return up256(sizeof(float) * M) + up256(sizeof(float2) * static_cast<size_t>(M) * ((V + 127) / 128));
   const BwdPlan p = bwd_plan(M, H, V);
-  const size_t gather = M > kGatherRows ? 4 * up256(sizeof(int) * M) + 256 +
+  const size_t gather = gathers(M, H, V) ? 4 * up256(sizeof(int) * M) + 256 +
                                               up256(sizeof(__half) * static_cast<size_t>(M) * ((H + 7) / 8 * 8))
                                         : 0;
   return gather + up256(sizeof(__half) * static_cast<size_t>(M) * p.vc) +
@@ -476,16 +466,22 @@ cudaError_t lm_logprobs(const __half* x, const __half* E, const int* targets, fl
   set_pdl(false);
   cudaError_t e;
   if (!rows_ok(x, ldx) || !rows_ok(E, lde)) return cudaErrorInvalidValue;
-  if (M <= kFewRows && sizeof(float) * kFewRows * (H + 255) <= kFewSmem) {
-    slots = std::min(slots, kFewBlocks * gemm_num_sms());
-    e = (M == 1 ? few_rows<1> : few_rows<2>)(x, E, targets, M, H, V, ldx, lde, part, tgt_logit, slots, st);
+  if (M == 1 && sizeof(float) * (static_cast<size_t>(H) + 255) <= kOneSmem) {
+    slots = std::min(slots, kOneBlocks * gemm_num_sms());
+    e = one_row(x, E, targets, H, V, lde, part, tgt_logit, slots, st);
   } else {
-    e = gemm(Operand{x, M, H, ldx}, Operand{E, V, H, lde}, M, V, Epi::kLogProb, ea, err, st, 256);
+    e = gemm(Operand{x, M, H, ldx}, Operand{E, V, H, lde}, M, V, Epi::kLogProb, ea, err, st,
+             tile_width(M, V));
   }
   if (e != cudaSuccess) return e;
   set_pdl(true);
-  return launch_pdl(logprob_finish_kernel, (M + kRows - 1) / kRows, kRows * kWarps, 0, st, ea.part2, ea.tgt_logit,
-                    targets, x, E, M, H, V, ldx, lde, slots, logp, lse);
+  auto finish = [&](auto kern, int rb) {
+    int warps = rb;
+    while (warps < kWarps && warps * (32 / rb) < slots) warps *= 2;
+    return launch_pdl(kern, (M + rb - 1) / rb, 32 * warps, 0, st, ea.part2, ea.tgt_logit, targets, x, E, M, H, V, ldx,
+                      lde, slots, logp, lse);
+  };
+  return M <= 8 * gemm_num_sms() ? finish(logprob_finish_kernel<4>, 4) : finish(logprob_finish_kernel<32>, 32);
 }
 
 cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* targets, const float* lse,
@@ -504,7 +500,7 @@ cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* ta
   const int* m_rows = nullptr;
   const int* place = nullptr;
   int in_ldx = ldx;
-  if (M > kGatherRows) {
+  if (gathers(M, H, V)) {
     char* g = reinterpret_cast<char*>(acc) + up256(sizeof(float) * static_cast<size_t>(p.slabs) * p.slab_rows * p.ld_acc);
     const size_t ints = up256(sizeof(int) * M);
     int* list = reinterpret_cast<int*>(g);
@@ -536,7 +532,8 @@ cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* ta
     ea.vocab_off = v0;
     ea.out = pc;
     ea.ld_out = p.vc;
-    cudaError_t e = gemm(Operand{in_x, M, H, in_ldx}, Operand{Ec, n, H, lde}, M, n, Epi::kProbs, ea, err, st, 256);
+    cudaError_t e = gemm(Operand{in_x, M, H, in_ldx}, Operand{Ec, n, H, lde}, M, n, Epi::kProbs, ea, err, st,
+                         tile_width(M, n));
     if (e != cudaSuccess) return e;
     set_pdl(true);
     EpiArgs eb;
@@ -550,8 +547,13 @@ cudaError_t lm_logprobs_backward(const __half* x, const __half* E, const int* ta
     e = gemm(Operand{pc, M, n, p.vc}, Operand{Ec, H, n, lde, true}, M, H, Epi::kStoreF32, eb, err, st, 256);
     if (e != cudaSuccess) return e;
   }
-  return launch_pdl(logprob_dx_kernel, M, 256, 0, st, acc, p.slabs, p.slab_rows, p.ld_acc, place, x, ldx, E, lde, lse,
-                    dlogp, targets, H, V, scale, dx, lddx);
+  // columns a warp: 128, more while there are over 16 warps an SM
+  int cols = 128;
+  while (cols < H && static_cast<int64_t>(M) * ((H + cols - 1) / cols) > 16 * gemm_num_sms()) cols *= 2;
+  const int parts = (H + cols - 1) / cols;
+  const int64_t items = static_cast<int64_t>(M) * parts;
+  return launch_pdl(logprob_dx_kernel, static_cast<unsigned>((items + 7) / 8), 256, 0, st, acc, p.slabs, p.slab_rows,
+                    p.ld_acc, place, x, ldx, E, lde, lse, dlogp, targets, M, H, V, scale, dx, lddx, cols, parts);
 }
 
 cudaError_t ce_stream_logp(const float* part_ref, const float* part_sum, const float* tgt_logit, const int* targets,
