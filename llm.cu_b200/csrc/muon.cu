@@ -76,8 +76,8 @@ __device__ __forceinline__ void small_product(const double* A, const double* B, 
 // step: loading, G, the product with P and the update of w, without a word to
 // the other warps, so that the warps' loads and products overlap.
 constexpr int kCols = 32;
-constexpr int kScalar = 8;  // single elements a lane loads at once
-struct Chunk {
+template <int kScalar>  // single elements a lane loads at once where it loads single ones
+struct ChunkOf {
   int64_t base;  // its first element in the buffers
   int64_t row;   // wide: elements between rows
   float* u;      // its first column in shared memory, rows `pitch` apart
@@ -140,6 +140,9 @@ struct Chunk {
 // behind a multiple of 32).
 template <int KB, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) muon_kernel(const MuonArgs a) {
+  // where single elements are the exception, fewer at once: 8 cost the others 5 us in 25
+  constexpr int kScalar = VEC ? 2 : 8;
+  using Chunk = ChunkOf<kScalar>;
   constexpr int K = 8 * KB;
   constexpr int kBlocks = KB == 2 ? 3 : 1;  // 8 x 8 blocks of G's upper half
   extern __shared__ __align__(16) float u[];
