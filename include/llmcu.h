@@ -432,8 +432,9 @@ llmcu_status llmcu_lm_logprobs(const void* x, const void* E, const int32_t* targ
 /* Its gradient for the hidden states (the head is frozen): dx[m] = scale *
  * dlogp[m] * (E[t] - sum_v exp(x[m] . E[v] - lse[m]) E[v]) as fp16 [rows,
  * hidden] with row stride lddx; 0 where the target scores nothing, whatever
- * dlogp holds there, and where dlogp is 0 (such rows cost next to nothing).  lse is the forward's.  `scale` (a loss scale, a power of
- * two as a rule) keeps small gradients in fp16's range.  Workspace:
+ * dlogp holds there, and where dlogp is 0 (large calls leave such rows out of
+ * the products).  lse is the forward's.  `scale` (a loss scale, a power of two
+ * as a rule) keeps small gradients in fp16's range.  Workspace:
  * llmcu_lm_logprobs_workspace(rows, hidden, vocab, 1) bytes. */
 llmcu_status llmcu_lm_logprobs_bwd(const void* x, const void* E, const int32_t* targets, const float* lse,
                                    const float* dlogp, void* dx, int rows, int hidden, int vocab, int ldx, int lde,
@@ -543,8 +544,8 @@ llmcu_status llmcu_policy_forward_backward(llmcu_ctx* ctx, const int32_t* tokens
                                            const float* old_logp, const float* ref_logp, const float* advantages,
                                            int batch, int seq, const llmcu_policy_cfg* cfg, float* loss_out,
                                            float* stats);
-/* Muon update of every adapter matrix with the gradients in place, in one
- * launch.  Its momentum lies where AdamW keeps its first moment (so
+/* Muon update of every adapter matrix with the gradients in place, in at most
+ * four launches.  Its momentum lies where AdamW keeps its first moment (so
  * llmcu_save_adamw_state / llmcu_load_adamw_state carry it, and
  * llmcu_reset_optimizer clears it): do not mix the two without a reset. */
 llmcu_status llmcu_muon(llmcu_ctx* ctx, const llmcu_muon_cfg* cfg);

@@ -1585,7 +1585,7 @@ llmcu_status llmcu_score(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* t
   GemmWorkspaceScope gws(ctx);
   CK(cudaMemsetAsync(ctx->fx_cnt, 0, sizeof(int) * kFxCounters, ctx->st));
   LoraDims d = ctx->ld;
-  if (!adapters) d.scale = 0.f;  // merged weights W + 0 B A: the base model
+  if (!adapters) d.r = 0;  // nothing is merged into W, whatever the adapters hold
   CK(merge_adapters(ctx, d));
   set_pdl(true);
   CKS(forward_layers(ctx, batch, seq));

@@ -84,6 +84,25 @@ def test_score_matches_golden(llmcu, cuda_device):
     c.ctx.close()
 
 
+@pytest.mark.parametrize("targets", [0x0F, 0x7F])
+def test_base_score_does_not_read_the_adapters(llmcu, cuda_device, targets):
+    """Diverged adapters (NaN, infinite, past fp16's range) leave the reference model's score as it is."""
+    from oracle import golden as G
+    tok, tgt = G.make_tokens(G.CFG_TINY, 2, 40, 4)
+    ctx = llmcu.Context(llmcu.Model.tiny(), llmcu.Lora(4, 8.0, targets), llmcu.Run(2, 40))
+    ctx.init_base_synthetic(3)
+    ctx.init_lora_synthetic(4)
+    good = ctx.lora_dict()
+    want = ctx.score(tok, tgt, adapters=False)
+    assert np.isfinite(want).all()
+    for bad in (np.nan, np.inf, 1e6):
+        ctx.set_lora_dict({k: np.full_like(v, bad) for k, v in good.items()})
+        assert np.array_equal(want, ctx.score(tok, tgt, adapters=False))
+    ctx.set_lora_dict(good)
+    assert np.isfinite(ctx.score(tok, tgt)).all()
+    ctx.close()
+
+
 def test_score_leaves_the_step_as_it_was(llmcu, cuda_device):
     """A cross-entropy step gives the same bits with and without a base-model score before it."""
     c = Case(llmcu, deterministic=True)
