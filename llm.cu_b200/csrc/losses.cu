@@ -540,10 +540,12 @@ __device__ __forceinline__ int count16(const PolicyArgs& a, int64_t i, int64_t f
 
 // Means over rows: the rows' weights, 1 / (batch * scored tokens), into
 // weights[row] (one CTA or warp a row); else the scored tokens of everything, a
-// partial sum a CTA, into counts[0 .. gridDim.x).
+// partial sum a CTA, into counts[0 .. gridDim.x).  *ended = 0.
 __global__ void __launch_bounds__(kThreads)
-    policy_count_kernel(PolicyArgs a, int* __restrict__ counts, double* __restrict__ weights) {
+    policy_count_kernel(PolicyArgs a, int* __restrict__ counts, double* __restrict__ weights,
+                        unsigned* __restrict__ ended) {
   pdl_trigger();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ended = 0u;
   __shared__ int red[kThreads / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int n = 0;
@@ -586,12 +588,30 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-__global__ void __launch_bounds__(kThreads, kMainBlocks)
-    policy_main_kernel(PolicyArgs a, const int* __restrict__ counts, int n_counts, const double* __restrict__ weights,
-                       double* __restrict__ partial) {
+// The CTAs' partial sums, in order: loss, mean KL, share of clipped tokens, scored tokens.
+__device__ __forceinline__ void sum_partials(const double* partial, int n, double* red, float* stats) {
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int i = threadIdx.x; i < n; i += kThreads)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += __ldcg(partial + i * 4 + k);
+  block_sums(v, red);
+  if (threadIdx.x == 0) write_stats(v, stats);
+}
+__global__ void __launch_bounds__(kThreads) policy_stats_kernel(const double* __restrict__ partial, int n,
+                                                               float* __restrict__ stats) {
   pdl_trigger();
   pdl_wait();
   __shared__ double red[4 * 32];
+  sum_partials(partial, n, red, stats);
+}
+
+__global__ void __launch_bounds__(kThreads, kMainBlocks)
+    policy_main_kernel(PolicyArgs a, const int* __restrict__ counts, int n_counts, const double* __restrict__ weights,
+                       double* partial, unsigned* ended) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ double red[4 * 32];
+  __shared__ bool last;
   double weight = a.inv_norm;  // of every token, but for means over rows: of the sums
   if (a.agg == kPolicyTokenMean) {
     double n[1] = {0.0};
@@ -643,21 +663,17 @@ __global__ void __launch_bounds__(kThreads, kMainBlocks)
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) partial[blockIdx.x * 4 + k] = v[k];
+    if (ended) {
+      __threadfence();
+      last = atomicAdd(ended, 1u) + 1u == gridDim.x;
+    }
   }
-}
-
-// The CTAs' partial sums, in order: loss, mean KL, share of clipped tokens, scored tokens.
-__global__ void __launch_bounds__(kThreads) policy_stats_kernel(const double* __restrict__ partial, int n,
-                                                               float* __restrict__ stats) {
-  pdl_trigger();
-  pdl_wait();
-  __shared__ double red[4 * 32];
-  double v[4] = {0.0, 0.0, 0.0, 0.0};
-  for (int i = threadIdx.x; i < n; i += kThreads)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] += partial[i * 4 + k];
-  block_sums(v, red);
-  if (threadIdx.x == 0) write_stats(v, stats);
+  if (!ended) return;
+  __syncthreads();
+  if (last) {
+    __threadfence();
+    sum_partials(partial, gridDim.x, red, a.stats);
+  }
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -682,9 +698,11 @@ cudaError_t preference_loss(PreferenceArgs a, cudaStream_t st) {
   return launch_cluster(preference_kernel, static_cast<unsigned>(a.pairs) * C, kThreads, C, 0, st, false, a);
 }
 
+constexpr size_t kEndedBytes = 16;  // CTAs of the main kernel that have ended
+
 size_t policy_loss_workspace(int batch) {
   const size_t partial = sizeof(double) * 4 * kMainBlocks * static_cast<size_t>(gemm_num_sms());
-  return partial + std::max(sizeof(int) * kCountBlocks, sizeof(double) * static_cast<size_t>(batch));
+  return partial + kEndedBytes + std::max(sizeof(int) * kCountBlocks, sizeof(double) * static_cast<size_t>(batch));
 }
 
 cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
@@ -719,7 +737,9 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
     return launch_cluster(policy_small_kernel, C, nt, C, smem, st, false, a, C);
   }
   double* partial = static_cast<double*>(ws);
-  int* counts = reinterpret_cast<int*>(partial + 4 * kMainBlocks * static_cast<size_t>(gemm_num_sms()));
+  char* behind = reinterpret_cast<char*>(partial + 4 * kMainBlocks * static_cast<size_t>(gemm_num_sms()));
+  unsigned* ended = reinterpret_cast<unsigned*>(behind);
+  int* counts = reinterpret_cast<int*>(behind + kEndedBytes);
   double* weights = reinterpret_cast<double*>(counts);  // the one or the other
   const bool was = pdl_enabled();
   set_pdl(false);
@@ -731,13 +751,18 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
     n_counts = static_cast<int>(std::min<int64_t>(kCountBlocks, (a.units / 4 + kThreads - 1) / kThreads + 1));
   }
   if (n_counts) {
-    e = launch_pdl(policy_count_kernel, n_counts, kThreads, 0, st, a, counts, weights);
+    e = launch_pdl(policy_count_kernel, n_counts, kThreads, 0, st, a, counts, weights, ended);
     set_pdl(true);
   }
   const int blocks = policy_blocks(a.units);
-  if (e == cudaSuccess) e = launch_pdl(policy_main_kernel, blocks, kThreads, 0, st, a, counts, n_counts, weights, partial);
+  // The count has zeroed `ended`, by which the main kernel's last CTA knows itself and sums up: a launch less
+  // (64 x 2047: 17.2 us a call against 18.7, where the host's launches take longer than the kernels; replayed
+  // from a graph 8.5 against 8.2).  Without a count a kernel of its own sums up.
+  if (e == cudaSuccess)
+    e = launch_pdl(policy_main_kernel, blocks, kThreads, 0, st, a, counts, n_counts, weights, partial,
+                   n_counts ? ended : nullptr);
   set_pdl(true);
-  if (e == cudaSuccess) e = launch_pdl(policy_stats_kernel, 1, kThreads, 0, st, partial, blocks, a.stats);
+  if (e == cudaSuccess && !n_counts) e = launch_pdl(policy_stats_kernel, 1, kThreads, 0, st, partial, blocks, a.stats);
   set_pdl(was);
   return e;
 }
