@@ -317,7 +317,7 @@ __device__ __forceinline__ void exp_rest2(const float (&x)[2], float (&rest)[2],
     if (!(fabsf(x[j]) < 1.f)) {
       ex[j] = expf(x[j]);
       em1[j] = ex[j] - 1.f;
-      rest[j] = em1[j] - x[j];
+      rest[j] = ex[j] < INFINITY ? em1[j] - x[j] : ex[j];  // also where x itself is infinite
     }
   }
 }
@@ -357,8 +357,10 @@ __device__ __forceinline__ void policy_tokens(const PolicyArgs& a, const float (
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       t[j].kl = kl[j];
-      t[j].grad = fmaf(-a.beta, em1[j], t[j].grad);
-      t[j].loss = fmaf(a.beta, kl[j], t[j].loss);
+      if (a.beta > 0.f) {  // else a statistic alone: an infinite term times 0 would be NaN
+        t[j].grad = fmaf(-a.beta, em1[j], t[j].grad);
+        t[j].loss = fmaf(a.beta, kl[j], t[j].loss);
+      }
     }
   }
 }

@@ -1,0 +1,65 @@
+"""The preference-tuning operators at the ends of their ranges: log-ratios whose
+exponential leaves 32 bits, infinite log-probabilities of scored tokens, logits
+past what the tensor cores resolve, and more than one vocabulary chunk."""
+
+import numpy as np
+import pytest
+import test_gpu_preference_ops as ops
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+U = ops.U
+# one launch; the count and the main kernel (means), the main kernel and the sums (a constant divisor)
+POLICY_CASES = [(8, 40, 43, 0), (8, 40, 43, 1), (8, 40, 43, 2), (40, 1500, 1501, 0), (40, 1500, 1501, 1),
+                (40, 1500, 1501, 2)]
+
+
+def policy_case(dev, B, S, ld, agg, seed):
+    lp, old, rf, adv, mask = ops.policy_inputs(dev, B, S, ld, seed, True, empty=(1,))
+    mask[:, ::7] = True  # the tokens that a test moves
+    junk = mask & ~(lp.isfinite() & old.isfinite() & rf.isfinite() & (lp > -1e30) & (old > -1e30) & (rf > -1e30))
+    return (*(torch.where(junk, -1.0, v) for v in (lp, old, rf)), adv, mask)
+
+
+@pytest.mark.parametrize("B,S,ld,agg", POLICY_CASES)
+def test_policy_without_kl_takes_any_reference(llmcu, cuda_device, B, S, ld, agg):
+    """kl_beta 0: the reference reaches the KL statistic alone, whatever it holds."""
+    lp, old, rf, adv, mask = policy_case(cuda_device, B, S, ld, agg, 3)
+    cfg = llmcu.Policy(0.2, 0.28, 0.0, 3.0, agg, 0.7 * B * S, True)
+    want = ops.run_policy(llmcu, cfg, lp, old, None, adv, mask, B, S, ld, cuda_device)
+    assert want[0].isfinite().all()
+    for far in (90.0, 200.0, 1000.0, float("inf"), float("-inf")):
+        rf[:, 7] = lp[:, 7] + far
+        rf[:, 14] = 0.0
+        stats, d = ops.run_policy(llmcu, cfg, lp, old, rf, adv, mask, B, S, ld, cuda_device)
+        assert torch.equal(d, want[1])
+        assert torch.equal(stats[[0, 2, 3]], want[0][[0, 2, 3]])
+        assert stats[1] > 1e30
+
+
+# ------------------------------------------------------------- on a context
+def context(llmcu, **run):
+    from oracle import golden as G
+    tok, tgt = G.make_tokens(G.CFG_TINY, 2, 40, 4)
+    ctx = llmcu.Context(llmcu.Model.tiny(), llmcu.Lora(4, 8.0), llmcu.Run(2, 40, deterministic=True, **run))
+    ctx.init_base_synthetic(3)
+    ctx.init_lora_synthetic(4)
+    return ctx, tok, tgt
+
+
+def test_policy_step_without_kl_takes_any_reference(llmcu, cuda_device):
+    """The default Policy() has kl_beta 0: a far reference leaves loss and adapter gradients as they are."""
+    ctx, tok, tgt = context(llmcu)
+    old = ctx.score(tok, tgt)
+    adv = np.array([1.0, -0.5], np.float32)
+    loss, stats = ctx.policy_forward_backward(tok, tgt, old, adv, llmcu.Policy())
+    want = ctx.grads_dict()
+    ref = old.copy()
+    ref[0, 3], ref[1, 5] = old[0, 3] + 90, old[1, 5] + 200
+    got = ctx.policy_forward_backward(tok, tgt, old, adv, llmcu.Policy(), ref)
+    assert got[0] == loss and got[1]["clipped"] == stats["clipped"] and got[1]["kl"] > 1e30
+    grads = ctx.grads_dict()
+    assert all(np.array_equal(grads[k], want[k]) for k in want)
+    ctx.close()
