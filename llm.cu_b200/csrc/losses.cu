@@ -277,8 +277,15 @@ __global__ void __launch_bounds__(kThreads)
 // below 1 the series x^2 (1/2! + x/3! + ...) is summed, to x^12 / 12! (the next
 // term is under 2^-25 of the sum).
 //
+// e^x leaves fp32 at 88.7, where the advantage (0 among others), beta or the
+// weight may bring it back: a thread whose sums come to kHuge or more, or to NaN,
+// takes its tokens again in 64 bits (far_terms), after its loop, so that the
+// loop has neither tests nor registers for it (64-bit terms inside it cost 1024 x
+// 8192 1.4 to 5 us of 36).
+//
 // Two tokens go through the series together (fma.rn.f32x2): the kernel is short
 // of issue slots.
+constexpr double kHuge = 1e16;
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t v;
   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
@@ -458,6 +465,39 @@ struct PolicyQuad {
   }
 };
 
+// A quad's loss, KL terms and gradients in 64 bits.
+__device__ __forceinline__ void far_terms(const PolicyArgs& a, const PolicyUnit& p, uint32_t bits, double weight,
+                                          float (&g)[4], double& loss, double& kl) {
+#pragma unroll 1
+  for (int j = 0; j < 4; ++j) {
+    if (!((bits >> j) & 1)) continue;
+    const double lp = static_cast<double>(__ldg(a.logp + p.i + j));
+    const double A = static_cast<double>(__ldg(a.adv + (a.token_adv ? p.i + j : p.row)));
+    const double delta = lp - static_cast<double>(__ldg(a.old + p.i + j));
+    const bool above = delta > (A > 0.0 ? a.log_high : a.log_dual), below = delta < a.log_low;
+    double grad = 0.0;
+    if (A > 0.0 ? above : A < 0.0 && (above || below)) {
+      loss -= (1.0 + static_cast<double>(A > 0.0 ? a.high : below ? a.low : a.dual)) * A;
+    } else if (A != 0.0 || !(delta == delta)) {  // no advantage, no term, whatever the ratio (but NaN stays)
+      grad = -exp(delta) * A;
+      loss += grad;
+    }
+    if (a.ref) {
+      const double d = static_cast<double>(__ldg(a.ref + p.i + j)) - lp, u = expm1(d);
+      const double k = u < INFINITY ? u - d : u;  // u also where d itself is infinite
+      kl += k;
+      if (a.beta > 0.f) {
+        loss += static_cast<double>(a.beta) * k;
+        grad -= static_cast<double>(a.beta) * u;
+      }
+    }
+    const float out = static_cast<float>(grad * weight);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i == j) g[i] = out;
+  }
+}
+
 __device__ __forceinline__ void write_stats(const double (&v)[4], float* stats) {
   const double t = fmax(v[3], 1.0);
   stats[0] = static_cast<float>(v[0]);
@@ -518,6 +558,17 @@ __global__ void __launch_bounds__(kSmallThreads) policy_small_kernel(PolicyArgs 
   double l = 0.0, kl = 0.0;
   int clips = 0;
   if (bits) quad.run(a, bits, static_cast<float>(weight), g, l, kl, clips);
+  if (!(fabs(l) < kHuge && fabs(kl) < kHuge)) {
+    float far_g[4] = {0.f, 0.f, 0.f, 0.f};
+    double far_l = 0.0, far_kl = 0.0;
+    far_terms(a, p, bits, weight, far_g, far_l, far_kl);
+    kl = far_kl;
+    if (!(fabs(l) < kHuge)) {  // else the KL terms alone are far, with kl_beta 0
+      l = far_l;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = far_g[j];
+    }
+  }
   if (a.dlogp) p.store(a, g);
   double v[4] = {l * weight, kl, static_cast<double>(clips), static_cast<double>(__popc(bits))};
   block_sums(v, red);
@@ -657,6 +708,24 @@ __global__ void __launch_bounds__(kThreads, kMainBlocks)
       tokens += __popc(bits);
     }
     if (a.dlogp) p.store(a, g);
+  }
+  if (!(fabs(v[0]) < kHuge && fabs(v[1]) < kHuge)) {
+    const bool all = !(fabs(v[0]) < kHuge);  // else the KL terms alone are far, with kl_beta 0
+    if (all) v[0] = 0.0;
+    v[1] = 0.0;
+#pragma unroll 1
+    for (u = blockIdx.x * run + threadIdx.x; u < u_end; u += kThreads) {
+      const PolicyUnit p(a, u);
+      const uint32_t bits = p.mask(a);
+      if (!bits) continue;
+      const double w = by_row ? weights[p.row] : weight;
+      float g[4] = {0.f, 0.f, 0.f, 0.f};
+      double l = 0.0;
+      far_terms(a, p, bits, w, g, l, v[1]);
+      if (!all) continue;
+      v[0] += by_row ? l * w : l;
+      if (a.dlogp) p.store(a, g);
+    }
   }
   v[0] *= weight;
   v[2] = static_cast<double>(clips);

@@ -39,6 +39,39 @@ def test_policy_without_kl_takes_any_reference(llmcu, cuda_device, B, S, ld, agg
         assert stats[1] > 1e30
 
 
+@pytest.mark.parametrize("B,S,ld,agg", POLICY_CASES)
+def test_policy_without_advantage_takes_any_ratio(llmcu, cuda_device, B, S, ld, agg):
+    """An advantage of 0 makes the ratio's terms 0, however far it lies off."""
+    lp, old, rf, adv, mask = policy_case(cuda_device, B, S, ld, agg, 4)
+    for col, far in ((7, 90.0), (14, 99.0), (21, 300.0), (28, -300.0)):
+        old[:, col] = lp[:, col] - far
+        adv[:, col] = 0.0
+    for dual in (0.0, 3.0):
+        cfg = llmcu.Policy(0.2, 0.28, 0.04, dual, agg, 0.7 * B * S, True)
+        ops.check_policy(llmcu, cfg, lp, old, rf, adv, mask, B, S, ld, cuda_device)
+    adv.zero_()
+    ops.check_policy(llmcu, cfg, lp, old, None, adv, mask, B, S, ld, cuda_device)
+    old[:, 7] = float("nan")  # NaN stays to be seen
+    stats, d = ops.run_policy(llmcu, cfg, lp, old, None, adv, mask, B, S, ld, cuda_device)
+    assert stats[0].isnan() and d[mask[:, 7], 7].isnan().all()
+
+
+@pytest.mark.parametrize("B,S,ld,agg", POLICY_CASES)
+@pytest.mark.parametrize("dual", [0.0, 3.0])
+def test_policy_exponentials_past_32_bits(llmcu, cuda_device, B, S, ld, agg, dual):
+    """e^90 is past fp32; kl_beta or the advantage, and the weight, bring it back."""
+    lp, old, rf, adv, mask = policy_case(cuda_device, B, S, ld, agg, 5)
+    for row, col, far in ((0, 7, 90.0), (2, 14, 92.5), (3, 21, 88.5), (4, 7, 41.0), (5, 14, 39.0)):
+        rf[row, col] = lp[row, col] + far
+        old[row, col + 7] = lp[row, col + 7] - far
+        adv[row, col + 7] = (1, -1)[row & 1] * 1e-4
+    # both at once, one of them tiny
+    rf[6, 7], old[6, 7] = lp[6, 7] + 91.0, lp[6, 7] - 1e-3
+    rf[7, 7], old[7, 7], adv[7, 7] = lp[7, 7] + 1e-3, lp[7, 7] - 91.0, -1e-5
+    cfg = llmcu.Policy(0.2, 0.28, 0.002, dual, agg, 0.7 * B * S, True)
+    ops.check_policy(llmcu, cfg, lp, old, rf, adv, mask, B, S, ld, cuda_device)
+
+
 # ------------------------------------------------------------- on a context
 def context(llmcu, **run):
     from oracle import golden as G
