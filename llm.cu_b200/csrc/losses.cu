@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(kThreads)
     if (a.kind == kPrefSigmoid) {
       const float e = a.smoothing, z = expf(-fabsf(h));
       const float l1 = log1pf(z);  // log(1 + e^x) = max(x, 0) + log1p(e^-|x|)
-      loss = (1.f - e) * (fmaxf(-h, 0.f) + l1) + e * (fmaxf(h, 0.f) + l1);
+      loss = (1.f - e) * (fmaxf(-h, 0.f) + l1);
+      if (e > 0.f) loss += e * (fmaxf(h, 0.f) + l1);  // e = 0: h may be infinite
       const float s_neg = h >= 0.f ? z / (1.f + z) : 1.f / (1.f + z);  // s(-h)
       dD = a.beta * (e - s_neg);
     } else {

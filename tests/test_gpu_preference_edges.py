@@ -72,6 +72,28 @@ def test_policy_exponentials_past_32_bits(llmcu, cuda_device, B, S, ld, agg, dua
     ops.check_policy(llmcu, cfg, lp, old, rf, adv, mask, B, S, ld, cuda_device)
 
 
+@pytest.mark.parametrize("P,S", [(3, 5), (3, 9000)])
+def test_preference_banned_tokens(llmcu, cuda_device, P, S):
+    """A rejected sequence with a token of probability 0 is preferred without
+    bounds: no loss, no gradient.  A chosen one loses without bounds."""
+    dev = cuda_device
+    lp = -torch.rand(2 * P, S, device=dev)
+    lp[P, S // 2] = float("-inf")  # pair 0: rejected
+    lp[1, S // 3] = float("-inf")  # pair 1: chosen
+    cfg = llmcu.Preference(llmcu.PREF_SIGMOID, 0.5)
+    loss, reward, d = ops.run_pref(llmcu, cfg, lp, None, None, None, P, S, S, dev)
+    assert loss[0] == 0 and loss[1] == float("inf") and loss[2].isfinite()
+    assert reward[P] == float("-inf") and reward[1] == float("-inf")
+    assert (d[[0, P]] == 0).all()
+    up = torch.tensor(1.0, device=dev) / P
+    assert torch.equal(d[1], (-0.5 * up).expand(S)) and torch.equal(d[P + 1], (0.5 * up).expand(S))
+    # smoothed labels hold a share of the other outcome, whose loss has no bound
+    loss, _, d = ops.run_pref(llmcu, llmcu.Preference(llmcu.PREF_SIGMOID, 0.5, 0.1), lp, None, None, None, P, S, S, dev)
+    assert (loss[:2] == float("inf")).all() and d.isfinite().all()
+    loss, _, d = ops.run_pref(llmcu, llmcu.Preference(llmcu.PREF_HINGE, 0.5), lp, None, None, None, P, S, S, dev)
+    assert loss[0] == 0 and loss[1] == float("inf") and (d[[0, P]] == 0).all()
+
+
 # ------------------------------------------------------------- on a context
 def context(llmcu, **run):
     from oracle import golden as G
