@@ -49,6 +49,20 @@ __device__ __forceinline__ float target_logit(const __half* __restrict__ x, cons
   return warp_sum(s);
 }
 
+// The pair p with one of its terms, the logit `rough`, replaced by `exact`.
+__device__ __forceinline__ float2 replace_term(float2 p, float rough, float exact) {
+  const float d = exact - rough;
+  if (fabsf(d) < 1.f) {
+    p.y = fmaf(exp2f((rough - p.x) * kLog2e), expm1f(d), p.y);
+  } else if (isfinite(d)) {
+    // logits of 1e5 and more, whose roundings pass 1: what is left without the
+    // term (nothing, where it was nearly all), joined with it
+    const float rest = p.y - exp2f((rough - p.x) * kLog2e);
+    p = rest > 1e-6f * p.y ? join_pairs(make_float2(p.x, rest), make_float2(exact, 1.f)) : make_float2(exact, 1.f);
+  }
+  return p;
+}
+
 constexpr int kWarps = 32;  // of the forward's finishing kernel: they share the slots
 
 // One row: the vocabulary is read once by plain loads and multiplied on the
@@ -200,12 +214,8 @@ __global__ void __launch_bounds__(32 * kWarps)
   for (int o = 16; o > 0; o >>= 1)
     p = join_pairs(p, make_float2(__shfl_xor_sync(0xffffffffu, p.x, o), __shfl_xor_sync(0xffffffffu, p.y, o)));
   if (lane == 0) {
-    float s = p.y;
-    if (ok) {
-      const float rough = tgt_logit[row], d = exact - rough;
-      if (isfinite(d)) s = fmaf(exp2f((rough - p.x) * kLog2e), expm1f(d), s);
-    }
-    const float ls = logf(s);
+    if (ok) p = replace_term(p, tgt_logit[row], exact);
+    const float ls = logf(p.y);
     lse[row] = p.x + ls;
     logp[row] = ok ? (exact - p.x) - ls : 0.f;  // not through lse, whose rounding a confident token would show
   }
@@ -239,9 +249,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps)
   for (int i = lane; i < slots; i += 32) s += ps[i] * exp2f((pr[i] - mx) * kLog2e);
   s = warp_sum(s);
   if (lane == 0) {
-    const float rough = tgt_logit[m], d = exact - rough;
-    if (isfinite(d)) s = fmaf(exp2f((rough - mx) * kLog2e), expm1f(d), s);
-    logp[m] = (exact - mx) - logf(s);
+    const float2 p = replace_term(make_float2(mx, s), tgt_logit[m], exact);
+    logp[m] = (exact - p.x) - logf(p.y);
   }
 }
 

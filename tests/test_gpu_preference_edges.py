@@ -94,6 +94,31 @@ def test_preference_banned_tokens(llmcu, cuda_device, P, S):
     assert loss[0] == 0 and loss[1] == float("inf") and (d[[0, P]] == 0).all()
 
 
+@pytest.mark.parametrize("M", [1, 5, 300])
+@pytest.mark.parametrize("sign", [1, -1, 0])
+def test_lm_logprobs_logits_past_their_rounding(llmcu, cuda_device, M, sign):
+    """Logits of millions, whose roundings pass 100: the results are off by the
+    logits' roundings and no more."""
+    dev, H, V = cuda_device, 2048, 700
+    g = torch.Generator(device=dev).manual_seed(M)
+    x = torch.randn(M, H, generator=g, device=dev) * 1000
+    E = torch.randn(V, H, generator=g, device=dev) * 100
+    if sign:
+        x, E = x.abs(), sign * E.abs()
+    x, E = x.half(), E.half()
+    z = x.double() @ E.double().t()
+    t = z.argmax(1).int()
+    t[1::2] = torch.randint(0, V, (M // 2,), generator=g, device=dev, dtype=torch.int32)
+    logp, lse = ops.lm_forward(llmcu, x, E, t)
+    ref = torch.logsumexp(z, 1)
+    tol = ops.logit_tol(x, E)
+    assert tol.min() > 100
+    lse_tol = tol + (64 + 4 * ref.abs() + 4 * z.abs().amax(1)) * U
+    ops.within(lse, ref, lse_tol)
+    ops.within(logp, z.gather(1, t.long()[:, None])[:, 0] - ref, lse_tol + tol + 2 * U * ref.abs())
+
+
+
 # ------------------------------------------------------------- on a context
 def context(llmcu, **run):
     from oracle import golden as G
