@@ -921,9 +921,10 @@ struct EpiLogProb {
 
 // Token log-probabilities, backward (lm_logprobs_backward), one vocabulary
 // chunk: 2^15 exp(l - lse) as fp16 into the chunk buffer (mapC).  lse is
-// known, so no value passes 2^15 and the factor keeps probabilities down to
-// 2^-29 (a uniform distribution over 150 k ids is at 2^-17) in fp16's normal
-// range.  The rounding to fp16 (at most 2^-11 of each value) is what the
+// known, so no value passes 2^15 (but for logits of 1e5 and more, which this
+// product rounds otherwise than the forward did by 0.7 and more: the conversion
+// saturates) and the factor keeps probabilities down to 2^-29 (a uniform
+// distribution over 150 k ids is at 2^-17) in fp16's normal range.  The rounding to fp16 (at most 2^-11 of each value) is what the
 // tensor cores' product with E needs; the target's column, whose p - 1 it
 // would spoil for a confident token, is stored as 0 and added in fp32 by the
 // finishing kernel.
@@ -967,7 +968,7 @@ struct EpiProbs {
             if (cj >= nv || cj == t) e0 = 0.f;
             if (cj + 1 >= nv || cj + 1 == t) e1 = 0.f;
           }
-          pk[16 * q + j / 2] = pack_half2(e0, e1);
+          pk[16 * q + j / 2] = pack_half2_sat(e0, e1);
         }
       }
       slab_wait_read(c);

@@ -366,6 +366,12 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
 }
+// The same with values past fp16's range brought to its largest (NaN stays).
+__device__ __forceinline__ uint32_t pack_half2_sat(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 
 // cp.async 16 B global -> shared; src_bytes = 0 zero-fills the destination.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int src_bytes) {

@@ -98,7 +98,8 @@ def test_preference_banned_tokens(llmcu, cuda_device, P, S):
 @pytest.mark.parametrize("sign", [1, -1, 0])
 def test_lm_logprobs_logits_past_their_rounding(llmcu, cuda_device, M, sign):
     """Logits of millions, whose roundings pass 100: the results are off by the
-    logits' roundings and no more."""
+    logits' roundings and no more, a probability is never over 1 by more than a
+    factor of two, and nothing is infinite."""
     dev, H, V = cuda_device, 2048, 700
     g = torch.Generator(device=dev).manual_seed(M)
     x = torch.randn(M, H, generator=g, device=dev) * 1000
@@ -116,7 +117,11 @@ def test_lm_logprobs_logits_past_their_rounding(llmcu, cuda_device, M, sign):
     lse_tol = tol + (64 + 4 * ref.abs() + 4 * z.abs().amax(1)) * U
     ops.within(lse, ref, lse_tol)
     ops.within(logp, z.gather(1, t.long()[:, None])[:, 0] - ref, lse_tol + tol + 2 * U * ref.abs())
-
+    dlogp = torch.ones(M, device=dev)
+    for slot in (t, (t + 1) % V):  # the likeliest column as the target and not
+        dx = ops.lm_backward(llmcu, x, E, slot, lse, dlogp, 1.0)
+        # (1 - p_t) E_t with 1 - p_t in [0, 1], and at most two columns near the top, each p at most 2
+        assert dx.isfinite().all() and (dx.abs() <= 5 * E.abs().max()).all()
 
 
 # ------------------------------------------------------------- on a context
