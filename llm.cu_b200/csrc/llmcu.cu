@@ -468,6 +468,9 @@ llmcu_status nccl_wait(llmcu_ctx* ctx, ncclResult_t r, const char* what) {
 }
 
 // Wait on the host for `ev` with the context deadline; on expiry abort NCCL.
+// Results are copied to the host after it: a copy into pageable memory blocks
+// until the stream has come to it, without a deadline.  The wait spins, as such
+// a copy does, so that the host learns of the end at once.
 llmcu_status wait_event(llmcu_ctx* ctx, cudaEvent_t ev) {
   const auto t0 = std::chrono::steady_clock::now();
   while (true) {
@@ -493,7 +496,7 @@ llmcu_status wait_event(llmcu_ctx* ctx, cudaEvent_t ev) {
       }
       return fail(ctx, LLMCU_ERR_TIMEOUT, "step did not complete within %d ms", ctx->timeout_ms);
     }
-    std::this_thread::sleep_for(std::chrono::microseconds(100));
+    std::this_thread::yield();
   }
 }
 
@@ -1122,10 +1125,10 @@ bool muon_args(const llmcu_muon_cfg* cfg, MuonArgs* a) {
 
 llmcu_status read_loss(llmcu_ctx* ctx, float* loss_out) {
   float h = 0.f;
-  CK(cudaMemcpyAsync(&h, ctx->loss_dev, sizeof(float), cudaMemcpyDeviceToHost, ctx->st));
   CK(cudaEventRecord(ctx->ev_step_done, ctx->st));
   CKS(wait_event(ctx, ctx->ev_step_done));
-  CKS(check_dev_err(ctx));
+  CK(cudaMemcpyAsync(&h, ctx->loss_dev, sizeof(float), cudaMemcpyDeviceToHost, ctx->st));
+  CKS(check_dev_err(ctx));  // waits for the copy too
   if (loss_out) *loss_out = h;
   return LLMCU_OK;
 }
@@ -1594,10 +1597,10 @@ llmcu_status llmcu_score(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* t
   TIMEDN(P_LMHEAD, 2, lm_logprobs(ctx->xf, ctx->E, ctx->tgt, ctx->tl_logp, ctx->lse_ce, M, H, ctx->V, H, H,
                                   reinterpret_cast<float2*>(ctx->part_ref), ctx->tgt_logit, ctx->derr, ctx->st));
   set_pdl(false);
-  CK(cudaMemcpyAsync(logp, ctx->tl_logp, sizeof(float) * M, cudaMemcpyDeviceToHost, ctx->st));
   CK(cudaEventRecord(ctx->ev_step_done, ctx->st));
   CKS(wait_event(ctx, ctx->ev_step_done));
-  return check_dev_err(ctx);
+  CK(cudaMemcpyAsync(logp, ctx->tl_logp, sizeof(float) * M, cudaMemcpyDeviceToHost, ctx->st));
+  return check_dev_err(ctx);  // waits for the copy too
 }
 
 llmcu_status llmcu_preference_forward_backward(llmcu_ctx* ctx, const int32_t* tokens, const int32_t* targets,

@@ -1,6 +1,8 @@
 """The preference-tuning operators at the ends of their ranges: log-ratios whose
 exponential leaves 32 bits, infinite log-probabilities of scored tokens, logits
 past what the tensor cores resolve, and more than one vocabulary chunk."""
+import ctypes as C
+import time
 
 import numpy as np
 import pytest
@@ -147,4 +149,37 @@ def test_policy_step_without_kl_takes_any_reference(llmcu, cuda_device):
     assert got[0] == loss and got[1]["clipped"] == stats["clipped"] and got[1]["kl"] > 1e30
     grads = ctx.grads_dict()
     assert all(np.array_equal(grads[k], want[k]) for k in want)
+    ctx.close()
+
+
+def busy(ctx, seconds):
+    """Keeps the context's stream from its next work for so long, on the host."""
+    nap = C.cast(C.CDLL(None).usleep, C.c_void_p)
+    launch = C.CDLL("libcuda.so.1").cuLaunchHostFunc
+    launch.argtypes = [C.c_void_p] * 3
+    assert launch(ctx.stream(), nap, int(seconds * 1e6)) == 0
+
+
+def test_score_and_steps_keep_their_deadline(llmcu, cuda_device):
+    """A stream that does not move within the deadline ends the call in time,
+    with nothing written behind its back; the context is usable again."""
+    TIMEOUT = 6
+    ctx, tok, tgt = context(llmcu)
+    adv = np.ones(2, np.float32)
+    old = ctx.score(tok, tgt)
+    calls = [lambda: ctx.score(tok, tgt), lambda: ctx.forward_backward(tok, tgt),
+             lambda: ctx.preference_forward_backward(tok, tgt, llmcu.Preference()),
+             lambda: ctx.policy_forward_backward(tok, tgt, old, adv, llmcu.Policy())]
+    for call in calls:
+        call()  # whatever a first call loads is there
+    for call in calls:
+        ctx.dp_set_timeout_ms(200)
+        busy(ctx, 1.5)
+        t0 = time.monotonic()
+        with pytest.raises(llmcu.LlmcuError) as e:
+            call()
+        assert e.value.status == TIMEOUT and time.monotonic() - t0 < 1.0
+        torch.cuda.synchronize()
+        ctx.dp_set_timeout_ms(60000)
+        assert np.array_equal(ctx.score(tok, tgt), old)
     ctx.close()
