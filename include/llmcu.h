@@ -186,7 +186,9 @@ llmcu_status llmcu_get_lora(llmcu_ctx* ctx, int layer, int proj, float* A, float
 llmcu_status llmcu_get_lora_grads(llmcu_ctx* ctx, int layer, int proj, float* dA, float* dB);
 /* Synthetic adapters on the device: A ~ U(+-1/sqrt(d_in)), B ~ N(0, b_std). */
 llmcu_status llmcu_init_lora_synthetic(llmcu_ctx* ctx, uint64_t seed, float b_std);
-/* Zero the AdamW moments (m, v). */
+/* Zero the optimizer's state: AdamW's moments (m, v), or Muon's momentum.  The
+ * two share their memory, and an update by the one is refused
+ * (LLMCU_ERR_INVALID_ARG) on the other's state until it is reset. */
 llmcu_status llmcu_reset_optimizer(llmcu_ctx* ctx);
 /* Total LoRA parameter count (A and B of every adapter). */
 int64_t llmcu_lora_param_count(const llmcu_ctx* ctx);
@@ -275,8 +277,9 @@ llmcu_status llmcu_generate(llmcu_ctx* ctx, const int32_t* prompt, int n_prompt,
 /* Optimizer sidecar for resuming (no reference counterpart: the reference
  * saves A / B only, src/train.cu:146-170): dir/lora_step{step}_adamw.bin holds
  * a 64-byte header ("LLMCUADW", version 1, step, layers, rank, hidden, q and
- * kv dims, parameter count) and the AdamW first and second moments, fp32, in
- * the flat adapter layout.  Together with llmcu_save_lora's A / B files of the
+ * kv dims, parameter count, the optimizer that the state is of) and the AdamW
+ * first and second moments (or Muon's momentum and zeros), fp32, in the flat
+ * adapter layout.  Together with llmcu_save_lora's A / B files of the
  * same step, llmcu_load_lora + llmcu_load_adamw_state restore the training
  * state; the next llmcu_train_step then takes step + 1.  Loading checks every
  * header field against the context (LLMCU_ERR_INVALID_ARG on a mismatch). */
@@ -547,7 +550,9 @@ llmcu_status llmcu_policy_forward_backward(llmcu_ctx* ctx, const int32_t* tokens
 /* Muon update of every adapter matrix with the gradients in place, in at most
  * four launches.  Its momentum lies where AdamW keeps its first moment (so
  * llmcu_save_adamw_state / llmcu_load_adamw_state carry it, and
- * llmcu_reset_optimizer clears it): do not mix the two without a reset. */
+ * llmcu_reset_optimizer clears it): on AdamW's moments, its own steps' or a
+ * loaded file's, the call is refused (LLMCU_ERR_INVALID_ARG), and so is AdamW
+ * on Muon's momentum. */
 llmcu_status llmcu_muon(llmcu_ctx* ctx, const llmcu_muon_cfg* cfg);
 
 #ifdef __cplusplus

@@ -77,6 +77,9 @@ struct LayerA {  // forward stash
 
 }  // namespace
 
+// whose state the optimizer's moments hold
+enum class Moments : int { kZero = 0, kAdamW = 1, kMuon = 2 };
+
 struct llmcu_ctx {
   llmcu_model_cfg m;
   llmcu_lora_cfg lc;
@@ -104,6 +107,7 @@ struct llmcu_ctx {
 
   // lora
   float *lp = nullptr, *lg = nullptr, *lm = nullptr, *lv = nullptr;
+  Moments moments = Moments::kZero;  // whose lm and lv are
   int lpart_amax = 0;
 
   // activations
@@ -1055,8 +1059,19 @@ llmcu_status validate_step(llmcu_ctx* ctx, int B, int S) {
   return LLMCU_OK;
 }
 
+// AdamW's first moment and Muon's momentum lie in the same place: neither may
+// go on from the other's.
+llmcu_status check_moments(llmcu_ctx* ctx, Moments who) {
+  if (ctx->moments == Moments::kZero || ctx->moments == who) return LLMCU_OK;
+  return fail(ctx, LLMCU_ERR_INVALID_ARG,
+              "the optimizer state is %s's: go on with that optimizer, or reset the state first (llmcu_reset_optimizer)",
+              ctx->moments == Moments::kAdamW ? "AdamW" : "Muon");
+}
+
 llmcu_status do_adamw(llmcu_ctx* ctx, const llmcu_adamw_cfg* o, int step) {
   if (!o || step < 1) return fail(ctx, LLMCU_ERR_INVALID_ARG, "adamw: null config or step < 1");
+  CKS(check_moments(ctx, Moments::kAdamW));
+  ctx->moments = Moments::kAdamW;
   const float bc1 = 1.0f - powf(o->beta1, static_cast<float>(step));
   const float bc2 = 1.0f - powf(o->beta2, static_cast<float>(step));
   TIMED(P_ADAMW, adamw_flat(ctx->lp, ctx->lg, ctx->lm, ctx->lv, ctx->n_lora, o->lr, o->beta1, o->beta2, o->eps, o->weight_decay,
@@ -1521,6 +1536,7 @@ llmcu_status llmcu_reset_optimizer(llmcu_ctx* ctx) {
   CK(cudaMemsetAsync(ctx->lm, 0, ctx->n_lora * sizeof(float), ctx->st));
   CK(cudaMemsetAsync(ctx->lv, 0, ctx->n_lora * sizeof(float), ctx->st));
   CK(cudaStreamSynchronize(ctx->st));
+  ctx->moments = Moments::kZero;
   return LLMCU_OK;
 }
 
@@ -1550,6 +1566,7 @@ llmcu_status llmcu_train_step(llmcu_ctx* ctx, const int32_t* tokens, const int32
   CK(cudaSetDevice(ctx->device));
   CKS(validate_step(ctx, batch, seq));
   if (!opt || step < 1) return fail(ctx, LLMCU_ERR_INVALID_ARG, "adamw: null config or step < 1");
+  CKS(check_moments(ctx, Moments::kAdamW));
   CKS(upload_tokens(ctx, tokens, targets, batch * seq));
   CKS(run_forward_backward(ctx, batch, seq));
   CKS(do_adamw(ctx, opt, step));
@@ -1562,6 +1579,7 @@ llmcu_status llmcu_train_step_device(llmcu_ctx* ctx, const int32_t* d_tokens, co
   CK(cudaSetDevice(ctx->device));
   CKS(validate_step(ctx, batch, seq));
   if (!opt || step < 1) return fail(ctx, LLMCU_ERR_INVALID_ARG, "adamw: null config or step < 1");
+  CKS(check_moments(ctx, Moments::kAdamW));
   const int M = batch * seq;
   CK(cudaMemcpyAsync(ctx->tok, d_tokens, sizeof(int) * M, cudaMemcpyDeviceToDevice, ctx->st));
   CK(cudaMemcpyAsync(ctx->tgt, d_targets, sizeof(int) * M, cudaMemcpyDeviceToDevice, ctx->st));
@@ -1655,6 +1673,8 @@ llmcu_status llmcu_muon(llmcu_ctx* ctx, const llmcu_muon_cfg* cfg) {
   MuonArgs a{};
   if (!muon_args(cfg, &a)) return fail(ctx, LLMCU_ERR_INVALID_ARG, "muon: invalid config");
   CK(cudaSetDevice(ctx->device));
+  CKS(check_moments(ctx, Moments::kMuon));
+  ctx->moments = Moments::kMuon;
   const LoraDims& d = ctx->ld;
   a.w = ctx->lp;
   a.grad = ctx->lg;
@@ -1949,7 +1969,8 @@ struct AdamwHeader {
   int32_t version, step, n_layers, rank, hidden, q_dim, kv_dim;
   int32_t targets;  // adapter mask; 0 reads as q/k/v/o
   int64_t n_params;
-  int64_t reserved2[2];
+  int64_t optimizer;  // Moments; older files hold 0 whoever wrote them
+  int64_t reserved;
 };
 static_assert(sizeof(AdamwHeader) == 64, "sidecar header is 64 bytes");
 constexpr char kAdamwMagic[8] = {'L', 'L', 'M', 'C', 'U', 'A', 'D', 'W'};
@@ -1977,6 +1998,7 @@ llmcu_status llmcu_save_adamw_state(llmcu_ctx* ctx, const char* dir, int step) {
   h.kv_dim = ctx->KV;
   h.targets = static_cast<int32_t>(ctx->ld.targets);
   h.n_params = ctx->n_lora;
+  h.optimizer = static_cast<int64_t>(ctx->moments);
   char path[1024];
   adamw_path(path, sizeof(path), dir, step);
   FILE* f = fopen(path, "wb");
@@ -2000,6 +2022,11 @@ llmcu_status llmcu_load_adamw_state(llmcu_ctx* ctx, const char* dir, int step) {
     return fail(ctx, LLMCU_ERR_IO, "%s is not an AdamW state file", path);
   }
   const uint32_t file_targets = h.targets ? static_cast<uint32_t>(h.targets) : kTargetsAttn;
+  if (h.optimizer < 0 || h.optimizer > static_cast<int64_t>(Moments::kMuon)) {
+    fclose(f);
+    return fail(ctx, LLMCU_ERR_INVALID_ARG, "%s holds the state of an unknown optimizer (%lld)", path,
+                static_cast<long long>(h.optimizer));
+  }
   if (h.step != step || h.n_layers != ctx->L || h.rank != ctx->ld.r || h.hidden != ctx->H || h.q_dim != ctx->Q ||
       h.kv_dim != ctx->KV || h.n_params != ctx->n_lora || file_targets != ctx->ld.targets) {
     fclose(f);
@@ -2015,6 +2042,14 @@ llmcu_status llmcu_load_adamw_state(llmcu_ctx* ctx, const char* dir, int step) {
   const bool ok = fread(m.data(), sizeof(float), n, f) == n && fread(v.data(), sizeof(float), n, f) == n;
   fclose(f);
   if (!ok) return fail(ctx, LLMCU_ERR_IO, "short read %s", path);
+  Moments who = static_cast<Moments>(h.optimizer);
+  if (who == Moments::kZero) {  // Muon leaves the second moment at zero, AdamW does not
+    const auto any = [](const std::vector<float>& x) {
+      return std::any_of(x.begin(), x.end(), [](float e) { return e != 0.f; });
+    };
+    who = any(v) ? Moments::kAdamW : any(m) ? Moments::kMuon : Moments::kZero;
+  }
+  ctx->moments = who;
   CK(cudaMemcpyAsync(ctx->lm, m.data(), n * sizeof(float), cudaMemcpyHostToDevice, ctx->st));
   CK(cudaMemcpyAsync(ctx->lv, v.data(), n * sizeof(float), cudaMemcpyHostToDevice, ctx->st));
   CK(cudaStreamSynchronize(ctx->st));

@@ -20,7 +20,8 @@
 // --int8-in-gemm (with --int8: the GEMMs stage the INT8 codes themselves),
 // --optimizer adamw|muon (default adamw; muon orthogonalises each adapter's
 // momentum, Nesterov, at 0.2 sqrt(max(rows, cols)), so that AdamW's learning
-// rates carry over; its momentum travels in the same sidecar).
+// rates carry over; its momentum travels in the same sidecar, and a run resumes
+// with the optimizer that wrote it).
 // Data parallel: when WORLD_SIZE > 1 (e.g. under torchrun) each process
 // drives GPU LOCAL_RANK, rank 0 writes the NCCL id to --dp-id-file and the
 // others read it; rank r takes sequences r, r+W, ... of every step window.

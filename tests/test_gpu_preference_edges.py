@@ -2,6 +2,8 @@
 exponential leaves 32 bits, infinite log-probabilities of scored tokens, logits
 past what the tensor cores resolve, and more than one vocabulary chunk."""
 import ctypes as C
+import os
+import subprocess
 import time
 
 import numpy as np
@@ -183,3 +185,65 @@ def test_score_and_steps_keep_their_deadline(llmcu, cuda_device):
         ctx.dp_set_timeout_ms(60000)
         assert np.array_equal(ctx.score(tok, tgt), old)
     ctx.close()
+
+
+def test_optimizers_do_not_take_each_others_moments(llmcu, cuda_device, tmp_path):
+    """AdamW's moments and Muon's momentum share their memory and their file; each is refused to the other."""
+    def refused(fn, *a):
+        with pytest.raises(llmcu.LlmcuError) as e:
+            fn(*a)
+        assert e.value.status == 1 and "reset" in str(e.value)
+
+    adamw, muon = llmcu.AdamW(), llmcu.Muon(lr=1e-3)
+    ctx, tok, tgt = context(llmcu)
+    ctx.forward_backward(tok, tgt)
+    start = ctx.lora_dict()
+    ctx.muon(muon)
+    after = ctx.lora_dict()
+    refused(ctx.adamw, adamw, 2)
+    refused(ctx.train_step, tok, tgt, adamw, 2)
+    assert all(np.array_equal(after[k], v) for k, v in ctx.lora_dict().items())
+    ctx.muon(muon)  # it goes on
+    ctx.save_adamw_state(str(tmp_path), 2)
+    ctx.reset_optimizer()
+    ctx.set_lora_dict(start)
+    ctx.train_step(tok, tgt, adamw, 1)
+    refused(ctx.muon, muon)
+    ctx.train_step(tok, tgt, adamw, 2)
+    ctx.save_adamw_state(str(tmp_path), 3)
+    ctx.load_adamw_state(str(tmp_path), 2)  # Muon's
+    refused(ctx.train_step, tok, tgt, adamw, 3)
+    ctx.muon(muon)
+    ctx.load_adamw_state(str(tmp_path), 3)  # AdamW's
+    refused(ctx.muon, muon)
+    ctx.train_step(tok, tgt, adamw, 4)
+    ctx.reset_optimizer()
+    ctx.muon(muon)
+    # files without the optimizer's number: AdamW's second moment tells whose they are
+    for step, mine, other in ((2, lambda: ctx.muon(muon), lambda: ctx.adamw(adamw, 3)),
+                              (3, lambda: ctx.adamw(adamw, 4), lambda: ctx.muon(muon))):
+        path = tmp_path / f"lora_step{step}_adamw.bin"
+        raw = bytearray(path.read_bytes())
+        raw[48:64] = bytes(16)
+        path.write_bytes(raw)
+        ctx.load_adamw_state(str(tmp_path), step)
+        refused(other)
+        mine()
+    ctx.close()
+
+
+@pytest.mark.parametrize("first,second", [("muon", "adamw"), ("adamw", "muon")])
+def test_llm_train_does_not_resume_across_optimizers(cuda_device, tmp_path, first, second):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = os.path.join(root, "llm.cu_b200", "llm_train")
+    args = [exe, "--config", "tiny", "--synthetic", "--seq-len", "32", "--batch", "1", "--save-every", "2",
+            "--log-every", "1", "--lr", "1e-3", "--out", str(tmp_path)]
+    one = subprocess.run(args + ["--steps", "2", "--optimizer", first], capture_output=True, text=True, timeout=120)
+    assert one.returncode == 0, one.stderr
+    two = subprocess.run(args + ["--steps", "3", "--resume", "2", "--optimizer", second], capture_output=True,
+                         text=True, timeout=120)
+    assert two.returncode != 0 and "reset" in two.stderr
+    assert not os.path.exists(tmp_path / "lora_step3_layer0_wq_A.bin")
+    same = subprocess.run(args + ["--steps", "3", "--resume", "2", "--optimizer", first], capture_output=True,
+                          text=True, timeout=120)
+    assert same.returncode == 0, same.stderr
