@@ -128,6 +128,74 @@ def test_lm_logprobs_logits_past_their_rounding(llmcu, cuda_device, M, sign):
         assert dx.isfinite().all() and (dx.abs() <= 5 * E.abs().max()).all()
 
 
+@pytest.mark.parametrize("M,H,V,chunks", [(4096, 64, 33000, 3), (9000, 8, 8000, 2), (4096, 64, 17000, 2),
+                                          (100, 8, 1300000, 2)])
+def test_lm_logprobs_backward_in_chunks(llmcu, cuda_device, M, H, V, chunks):
+    """Several vocabulary chunks, the last one narrower and with fewer K slices
+    than there are slabs; targets on both sides of every border.  The first shape
+    has over 2^33 products, so that the rows with a gradient are gathered first."""
+    dev = cuda_device
+    x, E, t = ops.lm_case(dev, M, H, V, 7)
+    # a chunk holds at most 2^26 probabilities in multiples of 1024 columns; its buffer shows in the workspace
+    width = max(1024, (1 << 26) // M // 1024 * 1024)
+    assert (V + width - 1) // width == chunks
+    assert 2 * M * width < llmcu.lm_logprobs_workspace(M, H, V, True) < 2 * M * V + 2 * M * width
+    border = [0, 1, V - 1, V - 2]
+    for c in range(1, chunks):
+        border += [c * width - 1, c * width, c * width + 1]
+    t[10:10 + len(border)] = torch.tensor(border, dtype=torch.int32, device=dev)
+    t[40::8], t[41] = -1, V
+    live = (t >= 0) & (t < V)
+    logp, lse = ops.lm_forward(llmcu, x, E, t)
+    dlogp = torch.randn(M, generator=torch.Generator(device=dev).manual_seed(2), device=dev)
+    dlogp[43::8] = 0
+    scale = 16.0
+    dx = ops.lm_backward(llmcu, x, E, t, lse, dlogp, scale)
+    assert torch.equal(dx, ops.lm_backward(llmcu, x, E, t, lse, dlogp, scale))
+    Ed = E.double()
+    for a in range(0, M, 1024):
+        r = slice(a, min(a + 1024, M))
+        z = x[r].double() @ Ed.t()
+        picked = z.gather(1, t[r].long().clamp(0, V - 1)[:, None])[:, 0]
+        p = torch.exp(z - lse[r].double()[:, None])
+        w = torch.where(live[r], scale * dlogp[r].double(), 0.0)[:, None]
+        Et = Ed[t[r].long().clamp(0, V - 1)]
+        want = w * (Et - p @ Ed)
+        # as for a single chunk, whose sums over K are in 32 bits too
+        tol = ops.logit_tol(x[r], E)
+        off = (tol + (8 + 4 * z.abs().amax(1) + 4 * lse[r].abs().double()) * U)[:, None]
+        pt = torch.exp(picked - lse[r].double())[:, None]
+        bound = w.abs() * ((p @ Ed.abs()) * (2.0 ** -11 + off + (V / 16 + 32) * 2 * U) +
+                           2.0 ** -40 * Ed.abs().sum(0)[None] + Et.abs() * (pt * off + 4 * U))
+        ops.within(dx[r], want, bound + want.abs() * (2.0 ** -11 + 8 * U) + 2.0 ** -25)
+    assert (dx[~live] == 0).all() and (dx[dlogp == 0] == 0).all()
+    assert llmcu.kernel_checks(ops.stream()) == 0
+
+
+@pytest.mark.parametrize("M,H,V", [(4096, 64, 33000), (9000, 8, 8000)])
+def test_lm_logprobs_backward_chunks_in_a_graph(llmcu, cuda_device, M, H, V):
+    """The chunks' buffer is used again and again under programmatic launch: the same bits from a captured call."""
+    dev = cuda_device
+    x, E, t = ops.lm_case(dev, M, H, V, 8)
+    t[5::9] = -1
+    _, lse = ops.lm_forward(llmcu, x, E, t)
+    dlogp = torch.randn(M, generator=torch.Generator(device=dev).manual_seed(2), device=dev)
+    want = ops.lm_backward(llmcu, x, E, t, lse, dlogp, 4.0)
+    n = llmcu.lm_logprobs_workspace(M, H, V, True)
+    ws, dx = torch.full((n,), 255, dtype=torch.uint8, device=dev), torch.zeros_like(want)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        llmcu.lm_logprobs_bwd(x.data_ptr(), E.data_ptr(), t.data_ptr(), lse.data_ptr(), dlogp.data_ptr(),
+                              dx.data_ptr(), M, H, V, H, H, H, 4.0, ws.data_ptr(), n, ops.stream())
+    for _ in range(3):
+        dx.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want)
+
+
 # ------------------------------------------------------------- on a context
 def context(llmcu, **run):
     from oracle import golden as G
