@@ -357,7 +357,8 @@ struct PolicyArgs {
   int div_s;
 };
 size_t policy_loss_workspace(int batch);
-cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st);
+// *launches (nullable): raised by the kernels launched (muon_update's too)
+cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st, int* launches = nullptr);
 
 // ---- muon.cu
 constexpr int kMuonMaxRank = 16;  // the smaller side of every matrix
@@ -381,6 +382,6 @@ struct MuonArgs {
   int cluster, tile, pitch;
   bool chained;  // not the first of its launches
 };
-cudaError_t muon_update(MuonArgs a, cudaStream_t st);
+cudaError_t muon_update(MuonArgs a, cudaStream_t st, int* launches = nullptr);
 
 }  // namespace llmcu

@@ -205,13 +205,16 @@ const char* kProfNames[P_COUNT] = {"gemm_tc", "attention_fwd", "attention_bwd", 
                                    "lora_merge", "lm_head", "embed", "adamw", "int8_dequant", "fill_and_loss",
                                    "dp_exposed"};
 
-// Records one event of a (begin, end) pair around `kernels` launches of class `cls`.
+// Records one event of a (begin, end) pair around `kernels` launches of class
+// `cls` (the end's number counts).
 void prof_mark(llmcu_ctx* c, int cls, int kernels = 1) {
   if (!c->prof_on || c->prof_n + 1 > static_cast<int>(c->prof_ev.size())) return;
   cudaEventRecord(c->prof_ev[c->prof_n], c->st);
   if ((c->prof_n & 1) == 0) {
     c->prof_cls.push_back(cls);
     c->prof_k.push_back(kernels);
+  } else {
+    c->prof_k.back() = kernels;
   }
   ++c->prof_n;
 }
@@ -684,8 +687,9 @@ struct TokenLoss {
 };
 
 // Loss and dL/dlogp of the step's log-probabilities (tl_logp), the gradients'
-// power of two (tl_norm) and the loss's sum at row_loss[M].
-llmcu_status run_token_loss(llmcu_ctx* ctx, const TokenLoss& tl, int B, int S) {
+// power of two (tl_norm) and the loss's sum at row_loss[M]; *launches raised by
+// the kernels launched.
+llmcu_status run_token_loss(llmcu_ctx* ctx, const TokenLoss& tl, int B, int S, int* launches) {
   cudaStream_t st = ctx->st;
   const int M = B * S;
   CK(ce_stream_logp(ctx->part_ref, ctx->part_sum, ctx->tgt_logit, ctx->tgt, ctx->xf, ctx->E, M, ctx->H, ctx->V,
@@ -700,6 +704,7 @@ llmcu_status run_token_loss(llmcu_ctx* ctx, const TokenLoss& tl, int B, int S) {
     a.pairs = B / 2;
     a.seq = a.ld = S;
     CK(preference_loss(a, st));
+    ++*launches;
     CK(loss_norm(ctx->tl_dlogp, M, ctx->tl_loss, a.pairs, ctx->tl_norm, ctx->row_loss + M, st));
   } else {
     PolicyArgs a = tl.policy;
@@ -711,9 +716,10 @@ llmcu_status run_token_loss(llmcu_ctx* ctx, const TokenLoss& tl, int B, int S) {
     a.dlogp = ctx->tl_dlogp;
     a.batch = B;
     a.seq = a.ld = S;
-    CK(policy_loss(a, ctx->tl_ws, st));
+    CK(policy_loss(a, ctx->tl_ws, st, launches));
     CK(loss_norm(ctx->tl_dlogp, M, ctx->tl_stats, 1, ctx->tl_norm, ctx->row_loss + M, st));
   }
+  *launches += 2;  // ce_stream_logp and loss_norm
   return LLMCU_OK;
 }
 
@@ -779,7 +785,7 @@ llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S, const TokenLoss*
         ctx->rc.deterministic
             ? 1
             : std::max(kLmSplitK, std::min(16, gemm_num_sms() / std::max(1, (M + 127) / 128 * ((H + 255) / 256))));
-    int launches = tl ? 5 : 2;  // + ce_stream_finish's two, or its one and about four of the loss
+    int launches = tl ? 1 : 2;  // + ce_stream_finish's two, or its one and the loss's (run_token_loss)
     for (int v0 = 0; v0 < V; v0 += (v0 == 0 ? vc0 : vc)) launches += 3;
     // one event pair around the whole section (per-kernel events would break
     // the programmatic-launch overlap of its short kernels)
@@ -809,7 +815,7 @@ llmcu_status run_forward_backward(llmcu_ctx* ctx, int B, int S, const TokenLoss*
       CK(gemm(op(ctx->pc, M, n, vc), op_mn(Ec, n, H, H), M, H, Epi::kStoreF32, eb, err, st));
       v0 += n;
     }
-    if (tl) CKS(run_token_loss(ctx, *tl, B, S));
+    if (tl) CKS(run_token_loss(ctx, *tl, B, S, &launches));
     CK(ce_stream_finish(ctx->part_ref, ctx->part_sum, ctx->tgt_logit, ctx->ce_ref, ctx->valid, ctx->tgt, E, M, H, V,
                         ctx->ce_slots, kGradScale, ctx->lse_ce, ctx->row_loss, ctx->d_xf, st,
                         tl ? ctx->tl_dlogp : nullptr, tl ? ctx->tl_norm : nullptr));
@@ -1686,7 +1692,8 @@ llmcu_status llmcu_muon(llmcu_ctx* ctx, const llmcu_muon_cfg* cfg) {
     a.slot[a.n_slots++] = MuonSlot{d.offA(p), d.r, d.d_in(p)};
     a.slot[a.n_slots++] = MuonSlot{d.offB(p), d.d_out(p), d.r};
   }
-  TIMED(P_ADAMW, muon_update(a, ctx->st));
+  int launches = 0;
+  TIMEDN(P_ADAMW, launches, muon_update(a, ctx->st, &launches));
   CK(cudaStreamSynchronize(ctx->st));
   return LLMCU_OK;
 }

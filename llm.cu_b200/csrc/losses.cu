@@ -777,7 +777,7 @@ size_t policy_loss_workspace(int batch) {
   return partial + kEndedBytes + std::max(sizeof(int) * kCountBlocks, sizeof(double) * static_cast<size_t>(batch));
 }
 
-cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
+cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st, int* launches) {
   a.vec16 = aligned(a.mask, 16);
   a.vec = aligned(a.logp, 16) && aligned(a.old, 16) && aligned(a.ref, 16) && aligned(a.mask, 4) &&
           aligned(a.dlogp, 16) && (!a.token_adv || aligned(a.adv, 16));
@@ -806,6 +806,7 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
     int C = 1;
     while (C * nt < a.units) C *= 2;
     const size_t smem = a.agg == kPolicySequenceMean ? sizeof(int) * C * a.batch : 0;
+    if (launches) ++*launches;
     return launch_cluster(policy_small_kernel, C, nt, C, smem, st, false, a, C);
   }
   double* partial = static_cast<double*>(ws);
@@ -827,6 +828,7 @@ cudaError_t policy_loss(PolicyArgs a, void* ws, cudaStream_t st) {
     set_pdl(true);
   }
   const int blocks = policy_blocks(a.units);
+  if (launches) *launches += 2;  // the count and the main kernel, or the main kernel and the sums
   // The count has zeroed `ended`, by which the main kernel's last CTA knows itself and sums up: a launch less
   // (64 x 2047: 17.2 us a call against 18.7, where the host's launches take longer than the kernels; replayed
   // from a graph 8.5 against 8.2).  Without a count a kernel of its own sums up.

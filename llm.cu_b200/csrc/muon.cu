@@ -457,7 +457,7 @@ bool vectors(const MuonArgs& a) {
 
 }  // namespace
 
-cudaError_t muon_update(MuonArgs all, cudaStream_t st) {
+cudaError_t muon_update(MuonArgs all, cudaStream_t st, int* launches) {
   if (all.n_slots < 1 || all.n_slots > kMuonMaxSlots || all.layers < 1 || all.steps < 1) return cudaErrorInvalidValue;
   auto long_side = [](const MuonSlot& s) { return std::max(s.rows, s.cols); };
   for (int i = 0; i < all.n_slots; ++i)
@@ -497,6 +497,7 @@ cudaError_t muon_update(MuonArgs all, cudaStream_t st) {
     const cudaError_t e = k <= 8 ? (vec ? launch<1, true>(a, st) : launch<1, false>(a, st))
                                  : (vec ? launch<2, true>(a, st) : launch<2, false>(a, st));
     if (e != cudaSuccess) return e;
+    if (launches) ++*launches;
     first = false;
   }
   return cudaSuccess;

@@ -2,6 +2,7 @@
 exponential leaves 32 bits, infinite log-probabilities of scored tokens, logits
 past what the tensor cores resolve, and more than one vocabulary chunk."""
 import ctypes as C
+import math
 import os
 import subprocess
 import time
@@ -298,6 +299,39 @@ def test_optimizers_do_not_take_each_others_moments(llmcu, cuda_device, tmp_path
         refused(other)
         mine()
     ctx.close()
+
+
+def test_profile_counts_the_launches(llmcu, cuda_device):
+    """Muon takes a launch for each cluster size, the losses one to two kernels beside the head's."""
+    from oracle import golden as G
+    m = llmcu.Model.tiny()
+    tok, tgt = G.make_tokens(G.CFG_TINY, 2, 40, 4)
+    old, adv = np.zeros((2, 40), np.float32), np.ones(2, np.float32)
+    for targets in (llmcu.TARGETS_ATTN, llmcu.TARGETS_ALL):
+        ctx = llmcu.Context(m, llmcu.Lora(4, 8.0, targets), llmcu.Run(2, 40))
+        ctx.init_base_synthetic(3)
+        ctx.init_lora_synthetic(4)
+        ctx.profile_enable()
+
+        def launches(kind, fn, *a):
+            ctx.profile_read()
+            fn(*a)
+            return ctx.profile_read()[kind]["launches"]
+
+        # 128 columns a CTA (few matrices), clusters of the next power of two up to eight
+        sides = {m.hidden, m.n_heads * m.head_dim, m.n_kv_heads * m.head_dim}
+        sides |= {m.ffn} if targets == llmcu.TARGETS_ALL else set()
+        clusters = {min(8, 1 << (math.ceil(s / 128) - 1).bit_length()) for s in sides}
+        ctx.forward_backward(tok, tgt)
+        assert launches("adamw", ctx.muon, llmcu.Muon(lr=1e-3)) == len(clusters)
+        ctx.reset_optimizer()
+        assert launches("adamw", ctx.adamw, llmcu.AdamW(), 1) == 1
+        # the cross-entropy finishes in two kernels; a loss in one of its own beside the
+        # log-probabilities, the gradients' scale and the finishing kernel
+        head = launches("lm_head", ctx.forward_backward, tok, tgt)
+        assert launches("lm_head", ctx.preference_forward_backward, tok, tgt, llmcu.Preference()) == head + 2
+        assert launches("lm_head", ctx.policy_forward_backward, tok, tgt, old, adv, llmcu.Policy()) == head + 2
+        ctx.close()
 
 
 @pytest.mark.parametrize("first,second", [("muon", "adamw"), ("adamw", "muon")])
