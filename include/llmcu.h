@@ -416,7 +416,12 @@ llmcu_status llmcu_attention_bwd_noalloc(const void* q, const void* k, const voi
  * 256-byte aligned (LLMCU_ERR_UNSUPPORTED otherwise).  Outputs must not overlap
  * inputs or the workspace (the Muon update works in place on w and momentum).
  * Sums run in a fixed order: the same call gives the same bits.  No reference
- * counterpart: the reference trains with the cross-entropy and AdamW only. */
+ * counterpart: the reference trains with the cross-entropy and AdamW only.
+ * Arithmetic: logits are the tensor cores' 32-bit sums of fp16 products (cut,
+ * not rounded, at each addition), the targets' and one row's are fp32 sums; the
+ * gradient's probabilities are rounded to fp16 (2^-11); logp - ref_logp, the
+ * policy's ratio and its KL terms are fp32, past fp32's range 64 bits; sums over
+ * tokens and Muon's small matrices are 64 bits. */
 
 /* Token log-probabilities of hidden states under a tied head, without logits
  * in memory: logp[m] = x[m] . E[t] - lse[m] with t = targets[m] and lse[m] =
@@ -493,7 +498,8 @@ typedef struct {
 size_t llmcu_policy_loss_workspace(int batch, int seq);
 /* Buffers [batch, seq] fp32 with row stride ld (>= seq); ref_logp may be null
  * (no KL term), mask as above.  stats (4 floats) receives the loss, the mean
- * of e^d - d - 1 over the scored tokens, the share of them that clip, and their
+ * of e^d - d - 1 over the scored tokens (whatever kl_beta; with 0 the reference
+ * reaches this number alone), the share of them that clip, and their
  * number (exact to 2^24); dlogp (nullable) the loss's gradient, 0 where nothing
  * is scored; columns from seq to ld are left as they are.  seq is at most 2^30
  * and batch * max(2, (seq + 6) / 4) below 2^31 (LLMCU_ERR_UNSUPPORTED). */
@@ -525,7 +531,10 @@ llmcu_status llmcu_muon_update(const llmcu_muon_cfg* cfg, float* w, const float*
  * scored (prompt, padding), and positions are scored whatever
  * llmcu_run_cfg.loss_all_positions says.  Log-probabilities are HOST fp32
  * [batch, seq]; what they hold where nothing is scored is not used.  Data
- * parallel: the gradients and the loss are averaged over ranks. */
+ * parallel: the gradients and the loss are averaged over ranks.  So
+ * LLMCU_POLICY_TOKEN_MEAN is then the mean of the ranks' token means (the mean
+ * over all scored tokens if each rank scores equally many), and
+ * LLMCU_POLICY_CONSTANT divides by norm times the number of ranks. */
 
 /* Log-probabilities of the targets (0 where not scored) under the current
  * adapters (adapters = 1) or the base alone (0: the reference model of the

@@ -152,10 +152,10 @@ struct EpiArgs {
   void* out = nullptr;
   int ld_out = 0;
   int accumulate = 0;
-  int ksplit = 1;  // kStoreF32 with accumulate: K slices that reduce-add into the same output
-  // kStoreF32 with ksplit > 1: rows between the K slices' own outputs (a
-  // multiple of 256; out then has ksplit * slab_rows rows and each element one
-  // writer, so the sums' order is fixed; no accumulate needed); 0: the same rows
+  int ksplit = 1;  // kStoreF32: K slices
+  // rows between the slices' own outputs (a multiple of 256; out then has ksplit
+  // * slab_rows rows and each element one writer, so the sums' order is fixed);
+  // 0: all reduce-add into the same rows (needs accumulate)
   int slab_rows = 0;
   const int* m_rows = nullptr;  // rows really there, on the device (null: M)
   // kStoreF16Delta: O [M, n_main] (row stride ld_o) and the delta output [B, n_heads, seq]

@@ -365,7 +365,7 @@ cudaError_t gemm(const Operand& A, const Operand& B, int M, int N, Epi epi, cons
   sh.b_scale = B.mn ? nullptr : B.q8_scale;
   sh.m_rows = ea.m_rows;
   sh.k_rotate = epi == Epi::kLogProb || epi == Epi::kProbs;
-  if (ea.ksplit > 1) {  // K slices reduce-add into the same rows
+  if (ea.ksplit > 1) {  // K slices: reduce-added into the same rows, or (slab_rows) each into rows of its own
     const int nk = sh.kb_per_split;
     const int kbps = (nk + ea.ksplit - 1) / ea.ksplit;
     sh.kb_per_split = kbps;

@@ -42,9 +42,9 @@ struct GemmShape {
   int M, N;
   int K;
   int tiles_m, tiles_n, num_tiles;
-  int splits;      // K splits (1 = none); split s writes rows [s * split_row_tiles * 128, ...)
+  int splits;      // K splits (1 = none); split s writes rows [s * split_row_tiles * rows per tile, ...)
   int kb_per_split;
-  int split_row_tiles;  // tiles_m: one row block of partials per split; 0: splits reduce-add into the same rows
+  int split_row_tiles;  // row tiles (of 128, or 256 for a CTA pair) between the splits' outputs; 0: all reduce-add into the same rows
   int n_fastest;        // tile order: 1 = consecutive units walk N (share A rows), 0 = walk M (share B)
   int n_main;           // columns [n_main, N) go to the side output
   __half* side;         // [M, N - n_main] fp16, row stride ld_side

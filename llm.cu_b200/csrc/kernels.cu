@@ -608,7 +608,8 @@ __global__ void scored_rows_kernel(uint8_t* __restrict__ mask, const int* __rest
 }
 
 // One CTA: norm[0] = the power of two that brings the largest |w[m]| into
-// [1/2, 1) (1 where all are 0, or one is not finite), norm[1] = 1 / norm[0] --
+// [1/2, 1) (1 where all are 0, or one is infinite; NaN is passed over, and
+// reaches the gradients by itself), norm[1] = 1 / norm[0] --
 // the fp16 backward then carries gradients of the size it does for the
 // cross-entropy, whatever the loss's scale; *total = the sum of loss[0 .. n)
 // in a fixed order.

@@ -67,9 +67,13 @@ constexpr int kWarps = 32;  // of the forward's finishing kernel: they share the
 
 // One row: the vocabulary is read once by plain loads and multiplied on the
 // CUDA cores, in fp32.  What bounds it is reading E: 622 MB for 151936 x 2048
-// is 95 us at the measured copy rate; with its finishing kernel it takes 103.
-// The GEMM takes 110 us there for one row as for sixteen, this kernel 113 for
-// two and 148 for four: the products would outweigh the loads.
+// is 95 us at the measured copy rate; with its finishing kernel it takes 103,
+// where the GEMM takes 120.  Smaller heads go the same way: 6.4 us against 7.2
+// for 128 x 64, 6.7 / 8.2 for 4096 x 256, 9.0 / 11.5 for 32000 x 256, 18.4 / 19.7
+// for 8192 x 2048, 35 / 44 for 40000 x 2048 (4096 x 2048 alone is 17.8 / 17.2).
+// From two rows on the GEMM takes all: there the products outweigh the loads (a
+// kernel like this one took 113 us for two rows and 148 for four at 151936 x
+// 2048, the GEMM 110).
 //
 // A warp takes four rows of E at a time, a lane eight elements of each every
 // 256; x lies in shared memory as fp32, its halves of eight apart, so that a
@@ -430,9 +434,10 @@ bool gathers(int M, int H, int V) {
 
 // Tile width of the products with the vocabulary: 256 columns, but up to 128
 // rows (one CTA a tile) 128 while these take one round: 77 rows of 872 x 3032
-// then take 12.3 us, else 16.  (With more rounds the wider tiles read E faster:
-// 16 rows of 2048 x 151936 take 121 us in five rounds of 256 columns, 141 in
-// nine of 128.)
+// then take 12.0 to 12.8 us, else 15.6 (near the full round they are even: 16
+// rows of 2048 x 18000 take 25.3 to 26.6 and 24.4).  With more rounds the wider
+// tiles read E faster: 16 rows of 2048 x 22000 take 26 us and 36 in tiles of 128,
+// of 2048 x 151936 110 in five rounds and 145 in nine.
 int tile_width(int M, int N) { return M <= 128 && (N + 127) / 128 <= gemm_num_sms() ? 128 : 256; }
 
 // rows for the TMA and for 16-byte loads
