@@ -329,7 +329,8 @@ struct PreferenceArgs {
   int pairs, seq, ld;
   int kind, mean_tokens;
   float beta, smoothing, margin;
-  bool vec;     // set by preference_loss: aligned bases
+  double still;  // set by preference_loss: with smoothing, the h whose gradient is 0
+  bool vec;      // set by preference_loss: aligned bases
   int cluster;  // set by preference_loss
 };
 cudaError_t preference_loss(PreferenceArgs a, cudaStream_t st);

@@ -225,8 +225,14 @@ __global__ void __launch_bounds__(kThreads)
       const float l1 = log1pf(z);  // log(1 + e^x) = max(x, 0) + log1p(e^-|x|)
       loss = (1.f - e) * (fmaxf(-h, 0.f) + l1);
       if (e > 0.f) loss += e * (fmaxf(h, 0.f) + l1);  // e = 0: h may be infinite
-      const float s_neg = h >= 0.f ? z / (1.f + z) : 1.f / (1.f + z);  // s(-h)
-      dD = a.beta * (e - s_neg);
+      if (e > 0.f) {
+        // e - s(-h) would cancel near the h whose gradient is 0; from t = h less
+        // that, e (1 - e) (e^t - 1) / (e + (1 - e) e^t), over e^t for t > 0
+        const float t = static_cast<float>(hd - a.still), u = expm1f(-fabsf(t)), v = expf(-fabsf(t)), f = 1.f - e;
+        dD = a.beta * e * f * (t > 0.f ? -u / fmaf(e, v, f) : u / fmaf(f, v, e));
+      } else {
+        dD = -a.beta * (h >= 0.f ? z / (1.f + z) : 1.f / (1.f + z));  // s(-h)
+      }
     } else {
       loss = hd < 1.0 ? static_cast<float>(1.0 - hd) : (hd >= 1.0 ? 0.f : h);  // NaN stays
       dD = hd < 1.0 ? -a.beta : (hd >= 1.0 ? 0.f : h);
@@ -767,6 +773,8 @@ cudaError_t preference_loss(PreferenceArgs a, cudaStream_t st) {
   const int quads = a.seq / 4 + 2;
   while (C < 8 && quads > 4 * C * kThreads && static_cast<int64_t>(a.pairs) * C < 8LL * gemm_num_sms()) C *= 2;
   a.cluster = C;
+  const double e = a.smoothing;
+  a.still = e > 0.0 ? std::log((1.0 - e) / e) : 0.0;
   return launch_cluster(preference_kernel, static_cast<unsigned>(a.pairs) * C, kThreads, C, 0, st, false, a);
 }
 

@@ -99,6 +99,35 @@ def test_preference_banned_tokens(llmcu, cuda_device, P, S):
     assert loss[0] == 0 and loss[1] == float("inf") and (d[[0, P]] == 0).all()
 
 
+@pytest.mark.parametrize("e", [0.01, 0.1, 0.3, 0.5])
+def test_preference_smoothed_gradient_near_its_zero(llmcu, cuda_device, e):
+    """Smoothed labels have a margin at which nothing pulls: the gradient keeps
+    its digits on both sides of it.  One token a row and no reference, so that h
+    is exact: off are t = h - h0 (rounded once, which moves e^t - 1 by at most
+    2 (1 + |t|) half steps), expm1f (2) and ten products and sums."""
+    dev = cuda_device
+    e = float(torch.tensor(e))
+    h0 = math.log((1 - e) / e)
+    t = torch.logspace(-7, 2.5, 200, dtype=torch.float64)
+    want_h = torch.cat([h0 - t, torch.tensor([h0]), h0 + t])
+    P = len(want_h)
+    cfg = llmcu.Preference(llmcu.PREF_SIGMOID, 0.5, e)
+    # D = chosen - rejected in two fp32 parts, whose difference 64 bits hold
+    D = want_h / 0.5
+    high = D.float()
+    lp = torch.cat([high, (high.double() - D).float()])[:, None].to(dev)
+    D = (lp[:P, 0].double() - lp[P:, 0].double()).cpu()
+    t = 0.5 * D - h0
+    _, _, d = ops.run_pref(llmcu, cfg, lp, None, None, torch.ones(P, device=dev), P, 1, 1, dev)
+    u, v = torch.expm1(-t.abs()), torch.exp(-t.abs())
+    want = 0.5 * e * (1 - e) * torch.where(t > 0, -u / (1 - e + e * v), u / (e + (1 - e) * v))
+    # the same as e - s(-h), as far as 64 bits tell them apart
+    assert ((0.5 * (e - torch.sigmoid(-0.5 * D)) - want).abs() <= 2.0 ** -50).all()
+    tol = (14 + 2 * t.abs().clamp(max=100)) * U * want.abs() + 2.0 ** -52
+    ops.within(d[:P, 0].cpu(), want, tol)
+    assert torch.equal(d[P:, 0], -d[:P, 0])
+
+
 @pytest.mark.parametrize("M", [1, 5, 300])
 @pytest.mark.parametrize("sign", [1, -1, 0])
 def test_lm_logprobs_logits_past_their_rounding(llmcu, cuda_device, M, sign):
