@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads)
         // e - s(-h) would cancel near the h whose gradient is 0; from t = h less
         // that, e (1 - e) (e^t - 1) / (e + (1 - e) e^t), over e^t for t > 0
         const float t = static_cast<float>(hd - a.still), u = expm1f(-fabsf(t)), v = expf(-fabsf(t)), f = 1.f - e;
-        dD = a.beta * e * f * (t > 0.f ? -u / fmaf(e, v, f) : u / fmaf(f, v, e));
+        dD = a.beta * f * (t > 0.f ? -e * u / fmaf(e, v, f) : e * u / fmaf(f, v, e));
       } else {
         dD = -a.beta * (h >= 0.f ? z / (1.f + z) : 1.f / (1.f + z));  // s(-h)
       }

@@ -99,7 +99,7 @@ def test_preference_banned_tokens(llmcu, cuda_device, P, S):
     assert loss[0] == 0 and loss[1] == float("inf") and (d[[0, P]] == 0).all()
 
 
-@pytest.mark.parametrize("e", [0.01, 0.1, 0.3, 0.5])
+@pytest.mark.parametrize("e", [1e-36, 1e-6, 0.01, 0.1, 0.3, 0.5])
 def test_preference_smoothed_gradient_near_its_zero(llmcu, cuda_device, e):
     """Smoothed labels have a margin at which nothing pulls: the gradient keeps
     its digits on both sides of it.  One token a row and no reference, so that h
